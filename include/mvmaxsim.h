@@ -32,7 +32,7 @@ typedef enum {
   MV_ERR_IO = -6         /* save/load failure */
 } mv_status;
 
-typedef enum { MV_F32 = 0, MV_BF16 = 1 } mv_dtype;
+typedef enum { MV_F32 = 0, MV_BF16 = 1, MV_F16 = 2 /* mv_enc_* operators only: rows and queries are MV_F32 or MV_BF16 */ } mv_dtype;
 
 /* Scoring modes of mv_query_topk / mv_score_all. */
 typedef enum {
@@ -466,6 +466,57 @@ MV_API int mv_enc_rmsnorm_bf16(int device, const void* d_x, const void* d_weight
                                float eps, float weight_offset, int style, void* stream);
 MV_API int mv_enc_gated_act_bf16(int device, const void* d_gate, int64_t gate_row_stride, const void* d_up, int64_t up_row_stride, void* d_out,
                                  int64_t rows, int64_t cols, int act, void* stream);
+
+/* Encoder operators (morphik_core_amd/encoder_attention.py): rotary positions with several axes and attention over key ranges, as the SigLIP /
+ * Gemma / Qwen2-VL blocks use them one behind the other.  DEVICE pointers, the caller's stream (0 = the null stream); enqueue-only, no
+ * allocation, so both may be captured into a graph.  Strides count elements.  Nothing is kept from one call for the next.
+ *
+ *   mv_enc_rotary  q [batch][rows][heads][dim] and k [batch][rows][kv_heads][dim] (either may have 0 heads) turned pair by pair:
+ *                  (x, y) -> scale * (x cos - y sin, y cos + x sin), x and y = elements (j, j + pairs), or (2 j, 2 j + 1) with adjacent != 0;
+ *                  elements from 2 * pairs on are copied.  Angle of pair j = positions[axis[j]] * inv_freq[j] in 64 bits, or cos / sin tables
+ *                  [batch][rows][pairs] by their strides (then positions must be NULL).  axis[j] must be an axis of positions.  Outputs may be the inputs
+ *                  themselves (same pointer, same strides).  dtype MV_F32, MV_BF16 or MV_F16; 16-byte vectors where pairs and strides allow. */
+typedef struct mv_rotary {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head;
+  int64_t q_out_batch, q_out_row, q_out_head, k_out_batch, k_out_row, k_out_head;
+  const void* positions; /* int32, or int64 with positions_are_64bit: [axes][batch][rows] by these strides */
+  int64_t positions_axis, positions_batch, positions_row;
+  const double* inv_freq; /* [pairs] */
+  const int32_t* axis;    /* [pairs] */
+  const float *cos, *sin;
+  int64_t table_batch, table_row, table_pair;
+  float scale;
+  int32_t dtype, positions_are_64bit, adjacent;
+  int32_t batch, rows, heads, kv_heads, dim, pairs;
+} mv_rotary;
+MV_API int mv_enc_rotary(int device, const mv_rotary* p, void* stream);
+
+/*   mv_enc_attention  out[b][i][h] = softmax_j(scale * q[b][i][h] . k[b][j][h / (heads / kv_heads)]) v[b][j][...] over the keys
+ *                  ranges[b][i][0] <= j < ranges[b][i][1] (cut to 0 .. keys; an empty range gives zeros; ranges NULL: every key).
+ *                  softcap c > 0: scores become c * tanh(score / c) first.  What keys outside a row's range hold does not reach the row,
+ *                  NaN and infinity included.  dtype MV_BF16 or MV_F16; dim a multiple of 8 up to 256; pointers 16-byte aligned (ranges: 8),
+ *                  strides multiples of 8 (ranges: 2, 0 = one for all); out contiguous [batch][rows][heads][dim].  Sums and softmax statistics
+ *                  are held in 32 bits, weights rounded to dtype for the product with v. */
+typedef struct mv_attn {
+  const void *q, *k, *v;
+  void* out;
+  const int32_t* ranges; /* [batch][rows][2] */
+  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head, ranges_batch;
+  int32_t dtype, batch, rows, keys, heads, kv_heads, dim;
+  float scale, softcap;
+} mv_attn;
+MV_API int mv_enc_attention(int device, const mv_attn* p, void* stream);
+
+/*   Key ranges.  A row at position i of a sequence [start, end) sees all of it (prefix < 0), or its first `prefix` keys and those up to i; a row
+ *                  outside its sequence sees nothing.  d_prefixes (nullable, one per sequence) overrides `prefix`; its negative values count as 0.
+ *   mv_enc_padded_ranges    batch entry b is the sequence [starts[b * starts_stride], ends[b * ends_stride]); row i stands at i + row_offset.
+ *   mv_enc_document_ranges  sequences packed one behind the other: document s is [offsets[s], offsets[s + 1]), offsets [docs + 1] ascending. */
+MV_API int mv_enc_padded_ranges(int device, const int32_t* d_starts, int64_t starts_stride, const int32_t* d_ends, int64_t ends_stride,
+                                const int32_t* d_prefixes, int32_t prefix, int32_t batch, int32_t rows, int64_t row_offset, int32_t* d_ranges, void* stream);
+MV_API int mv_enc_document_ranges(int device, const int32_t* d_offsets, int32_t docs, const int32_t* d_prefixes, int32_t prefix, int32_t rows,
+                                  int32_t* d_ranges, void* stream);
 
 /* Calibration: stream-read `bytes` of device memory `iters` times, returns average GB/s (measured peak
  * for the roofline denominator next to the 8 TB/s datasheet figure). */

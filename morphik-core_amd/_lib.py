@@ -72,7 +72,31 @@ class QueryStatsC(C.Structure):
     ]
 
 
+class RotaryC(C.Structure):
+    """mv_rotary: one call of mv_enc_rotary."""
+
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out")]
+        + [(n, C.c_int64) for n in ("q_batch", "q_row", "q_head", "k_batch", "k_row", "k_head", "q_out_batch", "q_out_row", "q_out_head", "k_out_batch",
+                                    "k_out_row", "k_out_head")]
+        + [("positions", C.c_void_p)] + [(n, C.c_int64) for n in ("positions_axis", "positions_batch", "positions_row")]
+        + [(n, C.c_void_p) for n in ("inv_freq", "axis", "cos", "sin")] + [("table_batch", C.c_int64), ("table_row", C.c_int64), ("table_pair", C.c_int64), ("scale", C.c_float)]
+        + [(n, C.c_int32) for n in ("dtype", "positions_are_64bit", "adjacent", "batch", "rows", "heads", "kv_heads", "dim", "pairs")]
+    )
+
+
+class AttnC(C.Structure):
+    """mv_attn: one call of mv_enc_attention."""
+
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("q", "k", "v", "out", "ranges")]
+        + [(n, C.c_int64) for n in ("q_batch", "q_row", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row", "v_head", "ranges_batch")]
+        + [(n, C.c_int32) for n in ("dtype", "batch", "rows", "keys", "heads", "kv_heads", "dim")] + [("scale", C.c_float), ("softcap", C.c_float)]
+    )
+
+
 MV_F32, MV_BF16 = 0, 1
+MV_F16 = 2  # mv_enc_* operators only
 MV_MODE_FLOAT, MV_MODE_BINARY, MV_MODE_FDE_THEN_FLOAT, MV_MODE_FDE_ONLY, MV_MODE_FLOAT_FP8, MV_MODE_FP8_THEN_FLOAT = 0, 1, 2, 3, 4, 5
 MV_WITH_FLOAT, MV_WITH_BINARY, MV_WITH_FDE, MV_WITH_FP8, MV_WITH_HOST_EXACT, MV_WITH_EXACT_SPLIT = 1, 2, 4, 8, 16, 32
 MV_WITH_FLOAT_LO = 64
@@ -112,7 +136,7 @@ EXPORTS = [
     "mv_comm_query_topk", "mv_comm_query_topk_batch", "mv_sign_pack", "mv_hamming_batch",
     "mv_index_import_fde", "mv_index_read_fde", "mv_query_topk_fde", "mv_query_topk_batch_fde", "mv_comm_query_topk_fde", "mv_comm_query_topk_batch_fde", "mv_two_stage_coarse_device_fde",
     "mv_fde_output_dim", "mv_fde_encode", "mv_calibrate_read_bw", "mv_calibrate", "mv_index_save", "mv_index_load",
-    "mv_enc_rmsnorm_bf16", "mv_enc_gated_act_bf16",
+    "mv_enc_rmsnorm_bf16", "mv_enc_gated_act_bf16", "mv_enc_rotary", "mv_enc_attention", "mv_enc_padded_ranges", "mv_enc_document_ranges",
 ]
 
 _lock = threading.Lock()
@@ -233,6 +257,10 @@ def lib() -> C.CDLL:
         L.mv_calibrate.argtypes = [C.c_int, C.c_int, i64, i32, C.POINTER(C.c_double)]
         L.mv_enc_rmsnorm_bf16.argtypes = [C.c_int, vp, vp, C.c_int, vp, i64, i32, C.c_float, C.c_float, C.c_int, vp]
         L.mv_enc_gated_act_bf16.argtypes = [C.c_int, vp, i64, vp, i64, vp, i64, i64, C.c_int, vp]
+        L.mv_enc_rotary.argtypes = [C.c_int, vp, vp]
+        L.mv_enc_attention.argtypes = [C.c_int, vp, vp]
+        L.mv_enc_padded_ranges.argtypes = [C.c_int, vp, i64, vp, i64, vp, i32, i32, i32, i64, vp, vp]
+        L.mv_enc_document_ranges.argtypes = [C.c_int, vp, i32, vp, i32, i32, vp, vp]
         L.mv_index_save.argtypes = [vp, C.c_char_p]
         L.mv_index_load.argtypes = [C.c_char_p, i32, C.POINTER(vp)]
         _lib = L

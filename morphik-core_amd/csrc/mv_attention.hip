@@ -24,7 +24,9 @@ using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using lds_u32x4 = __attribute__((address_space(3))) u32x4;
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -32,6 +34,8 @@ constexpr int kWaves = 4;
 constexpr int kWaveRows = 32;                  // rows of a wave: the N of the 32x32x16 matrix instruction
 constexpr int kBlockRows = kWaves * kWaveRows;
 constexpr float kRescale = 8.f;                // running maxima move only when a score passes them by 2^8: the weights stay <= 256
+
+constexpr int64_t kMaxRowStride = 1 << 23;    // elements: a tile's byte offsets stay below 2^31
 
 struct AttnArgs {
   const uint16_t *q, *k, *v;
@@ -51,8 +55,9 @@ __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {  // round to nearest even
-  if constexpr (BF16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-  else return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  const f32x2 v = {a, b};
+  if constexpr (BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 
 template <bool BF16>
@@ -104,21 +109,59 @@ __device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* 
     if (c * 64 + lane < a.dim) out[c * 64 + lane] = (uint16_t)pack2<BF16>(o[c] / l, 0.f);
 }
 
+// Where a 16-byte chunk of a staged row lies: chunk c of row r at r * CH + (c ^ swizzle(r)).  LDS serves 256 bytes a cycle: 16 lanes of a K read
+// (one row each, the same column) and 32 lanes of a V read (four rows x four chunks each) have to meet all 16 chunk positions.
+template <int CH>
+__device__ __forceinline__ int swizzle_k(int r) {
+  if constexpr (CH % 16 == 0) return r & 15;
+  else if constexpr (CH % 8 == 0) return (r >> 1) & 7;
+  else if constexpr (CH % 4 == 0) return (r >> 2) & 3;
+  else return (r >> 3) & 1;
+}
+template <int CH>
+__device__ __forceinline__ int swizzle_v(int r) {
+  if constexpr (CH % 16 == 0) return (r & 3) << 2;
+  else if constexpr (CH % 8 == 0) return ((r >> 1) & 1) << 2;
+  else return 0;
+}
+
+// 64 lanes x 16 bytes from base + offset (per lane) to 1 KiB of LDS at `slot`, without passing through registers; lanes off in exec leave their 16 bytes
+// alone.  The compiler does not count it: whoever reads the LDS waits with tile_barrier.
+__device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_t slot) {
+  uint32_t keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %1, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(offset), "s"(slot), "s"(base)
+      : "memory");
+}
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // One block: 128 rows against the keys that any of them sees, in tiles of BK keys staged through LDS.
 //
 // Scores are computed transposed, S^T = K Q^T: a lane then holds 16 keys of ONE row per 32 x 32 product, so the softmax is arithmetic within
 // the lane and one exchange with lane ^ 32.  The second product is transposed too, O^T = V^T P^T: its weight operand wants, per lane, eight
 // keys of one row -- the very registers the first product left, when V is read in the same order of keys.  V^T comes out of LDS by the
 // transposing read: 16 lanes that address four keys x 16 columns get one column each, four keys deep.
+//
+// Tiles are double-buffered: while one is computed the next is on its way from memory to LDS, and one barrier a tile both publishes the
+// arrived one and frees the other.
 template <bool BF16, int KC, int BK, bool CAP>
-__global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a) {
-  constexpr int DT = (KC + 1) / 2;           // 32-column tiles of the output; KC: 16-column steps of q.k
-  constexpr int CH = 2 * KC;                 // 16-byte chunks of a row
-  constexpr int KP = CH + 1, VP = CH + 4;    // LDS row pitches in chunks
-  __shared__ u32x4 lds_k[BK * KP];
-  __shared__ u32x4 lds_v[BK * VP];
+__global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArgs a) {
+  constexpr int DT = (KC + 1) / 2;             // 32-column tiles of the output; KC: 16-column steps of q.k
+  constexpr int CH = 2 * KC;                   // 16-byte chunks of a row
+  constexpr int VC = DT * 4;                   // and of a staged row of V (the last tile's unused columns hold anything: their results are dropped)
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kLoadsK = (BK * CH + kThreads - 1) / kThreads, kLoadsV = (BK * VC + kThreads - 1) / kThreads;
+  __shared__ __attribute__((aligned(1024))) u32x4 lds_k[2][BK * CH], lds_v[2][BK * VC];
   __shared__ int lds_range[kWaves][2];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
 
   int id = blockIdx.x;
   const int tile = id % a.tiles;
@@ -149,6 +192,7 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
     in_lo = max(in_lo, __shfl_xor(in_lo, s));
     in_hi = min(in_hi, __shfl_xor(in_hi, s));
   }
+  w_lo = uniform(w_lo), w_hi = uniform(w_hi), in_lo = uniform(in_lo), in_hi = uniform(in_hi);
   if (lane == 0) {
     lds_range[wave][0] = w_lo;
     lds_range[wave][1] = w_hi;
@@ -160,6 +204,7 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
     k_lo = min(k_lo, lds_range[w][0]);
     k_hi = max(k_hi, lds_range[w][1]);
   }
+  k_lo = uniform(k_lo), k_hi = uniform(k_hi);
 
   // q: the columns 16 kk + 8 half ... + 7 of this lane's row
   const uint16_t* qr = a.q + b * a.q_b + (int64_t)pos * a.q_l + head * a.q_h;
@@ -170,46 +215,80 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
     qf[kk] = live && c < a.dim ? *reinterpret_cast<const s16x8*>(qr + c) : s16x8{};
   }
 
+  // staging: thread t moves the chunks at positions t, t + 256, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
+  // one copies of the first (a row that is finite stays so; the weights and the columns of q there are zero)
+  const uint32_t k_step = (uint32_t)a.k_l * 2, v_step = (uint32_t)a.v_l * 2;
+  auto place = [&](int i, int n, int sw, uint32_t step, int last) {
+    const int row = i / n;
+    int c = i % n ^ sw;
+    c = c * 8 < a.dim ? c : 0;
+    return (uint32_t)min(row, last) * step + (uint32_t)c * 16;
+  };
+  uint32_t k_off[kLoadsK], v_off[kLoadsV];
+  auto offsets = [&](int last) {
+#pragma unroll
+    for (int n = 0; n < kLoadsK; ++n) k_off[n] = place(n * kThreads + threadIdx.x, CH, swizzle_k<CH>((n * kThreads + threadIdx.x) / CH), k_step, last);
+#pragma unroll
+    for (int n = 0; n < kLoadsV; ++n) v_off[n] = place(n * kThreads + threadIdx.x, VC, swizzle_v<VC>((n * kThreads + threadIdx.x) / VC), v_step, last);
+  };
+  offsets(BK);
+  auto fetch = [&](int k0, int buf) {
+    if (k0 + BK > k_hi) offsets(k_hi - 1 - k0);
+    const uint16_t* kt = kb + (int64_t)k0 * a.k_l;
+    const uint16_t* vt = vb + (int64_t)k0 * a.v_l;
+    const uint32_t dk = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_k[buf][wave * 64]), dv = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_v[buf][wave * 64]);
+#pragma unroll
+    for (int n = 0; n < kLoadsK; ++n)
+      if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH) dma16(kt, k_off[n], dk + n * kThreads * 16);
+#pragma unroll
+    for (int n = 0; n < kLoadsV; ++n)
+      if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC) dma16(vt, v_off[n], dv + n * kThreads * 16);
+  };
+
   f32x16 o[DT] = {};
   float m = -INFINITY, l = 0.f;
-  bool masked = false;
-  const uint16_t* lk = reinterpret_cast<const uint16_t*>(lds_k);
-  uint16_t* lv = reinterpret_cast<uint16_t*>(lds_v);
+  if (k_lo < k_hi) fetch(k_lo, 0);
 
-  for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < BK * CH; i += kWaves * 64) {
-      const int row = i / CH, c = i % CH, key = k0 + row;
-      const bool ok = key < k_hi && c * 8 < a.dim;
-      lds_k[row * KP + c] = ok ? *reinterpret_cast<const u32x4*>(kb + (int64_t)key * a.k_l + c * 8) : u32x4{};
-      lds_v[row * VP + c] = ok ? *reinterpret_cast<const u32x4*>(vb + (int64_t)key * a.v_l + c * 8) : u32x4{};
-    }
-    __syncthreads();
+  int buf = 0;
+  for (int k0 = k_lo; k0 < k_hi; k0 += BK, buf ^= 1) {
+    tile_barrier();
+    if (k0 + BK < k_hi) fetch(k0 + BK, buf ^ 1);
     if (k0 + BK <= w_lo || k0 >= w_hi) continue;  // nothing here for this wave
 
+    const uint16_t* lk = reinterpret_cast<const uint16_t*>(lds_k[buf]);
+    uint16_t* lv = reinterpret_cast<uint16_t*>(lds_v[buf]);
     f32x16 s[BK / 32] = {};
 #pragma unroll
-    for (int t = 0; t < BK / 32; ++t)
+    for (int t = 0; t < BK / 32; ++t) {
+      const int row = t * 32 + (lane & 31);
 #pragma unroll
       for (int kk = 0; kk < KC; ++kk)
-        s[t] = mfma<BF16>(*reinterpret_cast<const s16x8*>(lk + ((t * 32 + (lane & 31)) * KP + kk * 2 + half) * 8), qf[kk], s[t]);
+        s[t] = mfma<BF16>(*reinterpret_cast<const s16x8*>(lk + (row * CH + ((kk * 2 + half) ^ swizzle_k<CH>(row))) * 8), qf[kk], s[t]);
+    }
 
-    float top = -INFINITY;
-    const bool cut = k0 < in_lo || k0 + BK > in_hi;  // some row does not see some key of the tile
-    masked |= cut;
+    if constexpr (CAP) {
+#pragma unroll
+      for (int t = 0; t < BK / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = score<true>(s[t][e], a.qk, a.cap);
+    }
+    if (k0 < in_lo || k0 + BK > in_hi) {  // some row does not see some key of the tile
+#pragma unroll
+      for (int t = 0; t < BK / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + t * 32 + 8 * (e / 4) + 4 * half + e % 4;
+          s[t][e] = key >= lo && key < hi ? s[t][e] : -INFINITY;
+        }
+    }
+    float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float x = score<CAP>(s[t][e], a.qk, a.cap);
-        if (cut) {
-          const int key = k0 + t * 32 + 8 * (e / 4) + 4 * half + e % 4;
-          x = key >= lo && key < hi ? x : -INFINITY;
-        }
-        s[t][e] = x;
-        top = fmaxf(top, x);
-      }
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
     top = fmaxf(top, __shfl_xor(top, 32));
+    const float qk = CAP ? 1.f : a.qk;  // capped scores are logarithms already
+    top *= qk;
     if (__any(top > m + kRescale)) {
       const float m2 = fmaxf(m, top);
       const float alpha = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
@@ -230,7 +309,8 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
         u32x4 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[t][c * 8 + 2 * e] - base), y = __builtin_amdgcn_exp2f(s[t][c * 8 + 2 * e + 1] - base);
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][c * 8 + 2 * e], qk, -base));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][c * 8 + 2 * e + 1], qk, -base));
           l += x + y;
           w[e] = pack2<BF16>(x, y);
         }
@@ -241,9 +321,10 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
 #pragma unroll
       for (int c = 0; c < BK / 16; ++c) {
         // keys 16 c + 4 half + 0..3 and + 8..11 of column 32 d + (lane & 31)
-        uint16_t* src = lv + ((c * 16 + 4 * half + ((lane & 15) >> 2)) * VP * 8 + d * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+        const int row = c * 16 + 4 * half + ((lane & 15) >> 2), chunk = d * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        uint16_t* src = lv + (row * VC + (chunk ^ swizzle_v<VC>(row))) * 8 + 4 * (lane & 1);
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 8 * VP * 8));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 8 * VC * 8));
         o[d] = mfma<BF16>(__builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7), p[c], o[d]);
       }
   }
@@ -268,15 +349,13 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(const AttnArgs a
         *reinterpret_cast<u32x2*>(orow + c) = u32x2{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
       }
     }
-  if (masked) {
-    uint64_t again = __ballot(bad);
-    again = (again | again >> 32) & 0xffffffffu;
-    while (again) {
-      const int src = __builtin_ctzll(again);
-      again &= again - 1;
-      const int pos2 = __shfl(pos, src), head2 = __shfl(head, src), lo2 = __shfl(lo, src), hi2 = __shfl(hi, src);
-      exact_row<BF16, CAP>(a, a.q + b * a.q_b + (int64_t)pos2 * a.q_l + head2 * a.q_h, kb, vb, lo2, hi2, a.out + b * a.o_b + (int64_t)pos2 * a.o_l + head2 * a.o_h);
-    }
+  uint64_t again = __ballot(bad);
+  again = (again | again >> 32) & 0xffffffffu;
+  while (again) {
+    const int src = __builtin_ctzll(again);
+    again &= again - 1;
+    const int pos2 = __shfl(pos, src), head2 = __shfl(head, src), lo2 = __shfl(lo, src), hi2 = __shfl(hi, src);
+    exact_row<BF16, CAP>(a, a.q + b * a.q_b + (int64_t)pos2 * a.q_l + head2 * a.q_h, kb, vb, lo2, hi2, a.out + b * a.o_b + (int64_t)pos2 * a.o_l + head2 * a.o_h);
   }
 }
 
@@ -371,6 +450,10 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   }
   if (null || (all & 15) || (strides & 7) || (reinterpret_cast<uintptr_t>(p->ranges) & 7) || (p->ranges_batch & 1)) {
     set_error("mv_enc_attention: pointers must be set and 16-byte aligned, strides multiples of 8 elements");
+    return MV_ERR_INVALID;
+  }
+  if (p->k_row < 0 || p->k_row > kMaxRowStride || p->v_row < 0 || p->v_row > kMaxRowStride) {
+    set_error("mv_enc_attention: rows of k or v more than %lld elements apart", (long long)kMaxRowStride);
     return MV_ERR_INVALID;
   }
   AttnArgs a = {};

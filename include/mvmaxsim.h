@@ -498,15 +498,19 @@ MV_API int mv_enc_rotary(int device, const mv_rotary* p, void* stream);
  *                  softcap c > 0: scores become c * tanh(score / c) first.  What keys outside a row's range hold does not reach the row,
  *                  NaN and infinity included.  dtype MV_BF16 or MV_F16; dim a multiple of 8 up to 256; pointers 16-byte aligned (ranges: 8),
  *                  strides multiples of 8 (ranges: 2, 0 = one for all); out contiguous [batch][rows][heads][dim].  Sums and softmax statistics
- *                  are held in 32 bits, weights rounded to dtype for the product with v. */
+ *                  are held in 32 bits, weights rounded to dtype for the product with v.  Rows of k and v at most 2^23 elements apart.  Calls too small to
+ *                  fill the card are cut along the keys: their 32-bit sums pass through `workspace` and a second kernel joins them. */
 typedef struct mv_attn {
   const void *q, *k, *v;
   void* out;
   const int32_t* ranges; /* [batch][rows][2] */
   int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head, ranges_batch;
+  void* workspace; /* scratch for this call alone (16-byte aligned), may be NULL where mv_enc_attention_workspace_bytes says 0 */
+  int64_t workspace_bytes;
   int32_t dtype, batch, rows, keys, heads, kv_heads, dim;
   float scale, softcap;
 } mv_attn;
+MV_API int64_t mv_enc_attention_workspace_bytes(int device, int32_t batch, int32_t rows, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim);
 MV_API int mv_enc_attention(int device, const mv_attn* p, void* stream);
 
 /*   Key ranges.  A row at position i of a sequence [start, end) sees all of it (prefix < 0), or its first `prefix` keys and those up to i; a row

@@ -91,6 +91,7 @@ class AttnC(C.Structure):
     _fields_ = (
         [(n, C.c_void_p) for n in ("q", "k", "v", "out", "ranges")]
         + [(n, C.c_int64) for n in ("q_batch", "q_row", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row", "v_head", "ranges_batch")]
+        + [("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
         + [(n, C.c_int32) for n in ("dtype", "batch", "rows", "keys", "heads", "kv_heads", "dim")] + [("scale", C.c_float), ("softcap", C.c_float)]
     )
 
@@ -136,7 +137,7 @@ EXPORTS = [
     "mv_comm_query_topk", "mv_comm_query_topk_batch", "mv_sign_pack", "mv_hamming_batch",
     "mv_index_import_fde", "mv_index_read_fde", "mv_query_topk_fde", "mv_query_topk_batch_fde", "mv_comm_query_topk_fde", "mv_comm_query_topk_batch_fde", "mv_two_stage_coarse_device_fde",
     "mv_fde_output_dim", "mv_fde_encode", "mv_calibrate_read_bw", "mv_calibrate", "mv_index_save", "mv_index_load",
-    "mv_enc_rmsnorm_bf16", "mv_enc_gated_act_bf16", "mv_enc_rotary", "mv_enc_attention", "mv_enc_padded_ranges", "mv_enc_document_ranges",
+    "mv_enc_rmsnorm_bf16", "mv_enc_gated_act_bf16", "mv_enc_rotary", "mv_enc_attention", "mv_enc_attention_workspace_bytes", "mv_enc_padded_ranges", "mv_enc_document_ranges",
 ]
 
 _lock = threading.Lock()
@@ -259,6 +260,8 @@ def lib() -> C.CDLL:
         L.mv_enc_gated_act_bf16.argtypes = [C.c_int, vp, i64, vp, i64, vp, i64, i64, C.c_int, vp]
         L.mv_enc_rotary.argtypes = [C.c_int, vp, vp]
         L.mv_enc_attention.argtypes = [C.c_int, vp, vp]
+        L.mv_enc_attention_workspace_bytes.argtypes = [C.c_int, i32, i32, i32, i32, i32, i32]
+        L.mv_enc_attention_workspace_bytes.restype = C.c_int64
         L.mv_enc_padded_ranges.argtypes = [C.c_int, vp, i64, vp, i64, vp, i32, i32, i32, i64, vp, vp]
         L.mv_enc_document_ranges.argtypes = [C.c_int, vp, i32, vp, i32, i32, vp, vp]
         L.mv_index_save.argtypes = [vp, C.c_char_p]

@@ -8,6 +8,7 @@
 // packed one behind the other.  Heads that share a K/V head are rows of ONE problem (row r = position r / group, head r % group): K and V
 // are read once for all of them, and a single position still fills a matrix instruction.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "mv_common.h"
@@ -25,14 +26,24 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using lds_u32x4 = __attribute__((address_space(3))) u32x4;
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWaves = 4;
 constexpr int kWaveRows = 32;                  // rows of a wave: the N of the 32x32x16 matrix instruction
-constexpr int kBlockRows = kWaves * kWaveRows;
+constexpr int kXcds = 8;
+// By KC, the 16-column steps of a head.  Keys of a tile: two products deep where the registers allow it.  Waves of a SIMD at once: by registers.
+// Waves of a block: eight share a tile's loads (2 x 4096 rows, heads of 128: 278 us with four, 270 with eight; 4 x 2048 of 256: 163 and 146), but for
+// heads of 72 ... 96, whose tiles do not divide evenly among 512 threads and which vision towers use with short windows (heads of 80: 8464 rows 467 us
+// with four, 543 with eight; windows of 64 rows 64 and 78).
+constexpr int tile_keys(int kc) { return kc > 8 ? 32 : 64; }
+constexpr int waves_per_simd(int kc) { return kc <= 4 ? 4 : 2; }
+constexpr int block_waves(int kc) { return kc == 5 || kc == 6 ? 4 : 8; }
+constexpr int block_rows(int kc) { return block_waves(kc) * kWaveRows; }
+// The widths that are built: a head takes the next wider one
+constexpr int built_kc(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : dim <= 128 ? 8 : dim <= 192 ? 12 : 16; }
 constexpr float kRescale = 8.f;                // running maxima move only when a score passes them by 2^8: the weights stay <= 256
 
 constexpr int64_t kMaxRowStride = 1 << 23;    // elements: a tile's byte offsets stay below 2^31
@@ -42,7 +53,9 @@ struct AttnArgs {
   uint16_t* out;
   const int32_t* ranges;  // [batch or 1][rows][2] or null: every row sees every key
   int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, o_b, o_l, o_h, range_b;  // strides in elements
-  int32_t rows, keys, kv_heads, group, dim, tiles;  // tiles: blocks of kBlockRows over rows * group
+  int32_t rows, keys, kv_heads, group, dim, tiles, block_rows;  // tiles: blocks of block_rows over rows * group
+  int32_t full, splits;  // blocks [0, full) take a tile each; the tiles behind them are cut into `splits` runs of keys, one block each
+  float* partial;        // of those: [tile - full][split][rows of a tile] x (dim sums, maximum, sum of weights, 2 unused)
   float qk;    // scale * log2(e); with a cap: scale / cap * 2 log2(e)
   float cap;   // cap * log2(e), 0 = none
 };
@@ -81,7 +94,7 @@ __device__ __forceinline__ float score(float s, float qk, float cap) {
 // weight 0 of a masked key would carry that key's NaN or infinity into the row.  Rare by nature (only where masked places hold such values, or
 // where the row's own operands do), so it is simple rather than fast.
 template <bool BF16, bool CAP>
-__device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int lo, int hi, uint16_t* out) {
+__device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int lo, int hi, uint16_t* out, float* partial) {
   const int lane = threadIdx.x & 63;
   float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -106,7 +119,11 @@ __device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* 
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    if (c * 64 + lane < a.dim) out[c * 64 + lane] = (uint16_t)pack2<BF16>(o[c] / l, 0.f);
+    if (c * 64 + lane < a.dim) {
+      if (partial) partial[c * 64 + lane] = o[c];
+      else out[c * 64 + lane] = (uint16_t)pack2<BF16>(o[c] / l, 0.f);
+    }
+  if (partial && lane == 0) *reinterpret_cast<float2*>(partial + a.dim) = make_float2(m, l);
 }
 
 // Where a 16-byte chunk of a staged row lies: chunk c of row r at r * CH + (c ^ swizzle(r)).  LDS serves 256 bytes a cycle: 16 lanes of a K read
@@ -128,22 +145,19 @@ __device__ __forceinline__ int swizzle_v(int r) {
 // 64 lanes x 16 bytes from base + offset (per lane) to 1 KiB of LDS at `slot`, without passing through registers; lanes off in exec leave their 16 bytes
 // alone.  The compiler does not count it: whoever reads the LDS waits with tile_barrier.
 __device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_t slot) {
-  uint32_t keep;
   asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 4\n\t"
-      "global_load_lds_dwordx4 %1, %3\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(keep)
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %2"
+      :
       : "v"(offset), "s"(slot), "s"(base)
-      : "memory");
+      : "memory", "m0");
 }
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// One block: 128 rows against the keys that any of them sees, in tiles of BK keys staged through LDS.
+// One block: 32 rows a wave against the keys that any of them sees, in tiles of BK keys staged through LDS.
 //
 // Scores are computed transposed, S^T = K Q^T: a lane then holds 16 keys of ONE row per 32 x 32 product, so the softmax is arithmetic within
 // the lane and one exchange with lane ^ 32.  The second product is transposed too, O^T = V^T P^T: its weight operand wants, per lane, eight
@@ -152,8 +166,10 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 //
 // Tiles are double-buffered: while one is computed the next is on its way from memory to LDS, and one barrier a tile both publishes the
 // arrived one and frees the other.
-template <bool BF16, int KC, int BK, bool CAP>
-__global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArgs a) {
+template <bool BF16, int KC, bool CAP>
+__global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void attention_kernel(const AttnArgs a) {
+  constexpr int kWaves = block_waves(KC), kBlockRows = block_rows(KC);
+  constexpr int BK = tile_keys(KC);
   constexpr int DT = (KC + 1) / 2;             // 32-column tiles of the output; KC: 16-column steps of q.k
   constexpr int CH = 2 * KC;                   // 16-byte chunks of a row
   constexpr int VC = DT * 4;                   // and of a staged row of V (the last tile's unused columns hold anything: their results are dropped)
@@ -163,8 +179,20 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArg
   __shared__ int lds_range[kWaves][2];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
 
-  int id = blockIdx.x;
-  const int tile = id % a.tiles;
+  // Blocks of one K/V head next to each other on one XCD (its L2 then holds that head's keys once): consecutive block numbers go round the XCDs, so
+  // number x + 8 i becomes the i-th of XCD x's run.  The cut tiles, of equal length among themselves, are dealt out the same way behind the others.
+  const int run = blockIdx.x < a.full ? a.full : gridDim.x - a.full;
+  const int at = blockIdx.x < a.full ? blockIdx.x : blockIdx.x - a.full;
+  const int x = at & (kXcds - 1), each = run / kXcds, more = run % kXcds;
+  int id = x * each + min(x, more) + at / kXcds, split = 0;
+  float* partial = nullptr;
+  if (blockIdx.x >= a.full) {
+    split = id % a.splits;
+    id /= a.splits;
+    if (a.splits > 1) partial = a.partial + ((int64_t)id * a.splits + split) * min((int64_t)kBlockRows, (int64_t)a.rows * a.group) * (a.dim + 4);
+    id += a.full;
+  }
+  const int tile = a.tiles - 1 - id % a.tiles;  // the last rows first: under a causal mask they have the most to do
   id /= a.tiles;
   const int hk = id % a.kv_heads, b = id / a.kv_heads;
   const uint16_t* kb = a.k + b * a.k_b + hk * a.k_h;
@@ -205,6 +233,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArg
     k_hi = max(k_hi, lds_range[w][1]);
   }
   k_lo = uniform(k_lo), k_hi = uniform(k_hi);
+  int lo_s = lo, hi_s = hi;  // what this block sees of the row's range
+  if (partial) {
+    const int share = ((k_hi - k_lo + BK - 1) / BK + a.splits - 1) / a.splits * BK;  // whole tiles
+    k_lo = k_lo < k_hi ? (int)min((int64_t)k_lo + (int64_t)split * share, (int64_t)k_hi) : 0;
+    k_hi = min((int64_t)k_lo + share, (int64_t)k_hi);
+    lo_s = max(lo, k_lo), hi_s = min(hi, k_hi);
+  }
 
   // q: the columns 16 kk + 8 half ... + 7 of this lane's row
   const uint16_t* qr = a.q + b * a.q_b + (int64_t)pos * a.q_l + head * a.q_h;
@@ -215,7 +250,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArg
     qf[kk] = live && c < a.dim ? *reinterpret_cast<const s16x8*>(qr + c) : s16x8{};
   }
 
-  // staging: thread t moves the chunks at positions t, t + 256, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
+  // staging: thread t moves the chunks at positions t, t + kThreads, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
   // one copies of the first (a row that is finite stays so; the weights and the columns of q there are zero)
   const uint32_t k_step = (uint32_t)a.k_l * 2, v_step = (uint32_t)a.v_l * 2;
   auto place = [&](int i, int n, int sw, uint32_t step, int last) {
@@ -232,17 +267,20 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArg
     for (int n = 0; n < kLoadsV; ++n) v_off[n] = place(n * kThreads + threadIdx.x, VC, swizzle_v<VC>((n * kThreads + threadIdx.x) / VC), v_step, last);
   };
   offsets(BK);
+  const uint16_t *kt = kb + (int64_t)k_lo * a.k_l, *vt = vb + (int64_t)k_lo * a.v_l;  // of the tile sent for next
+  const int64_t kt_step = a.k_l * BK, vt_step = a.v_l * BK;
+  const uint32_t dk = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_k[0][wave * 64]), dv = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_v[0][wave * 64]);
   auto fetch = [&](int k0, int buf) {
     if (k0 + BK > k_hi) offsets(k_hi - 1 - k0);
-    const uint16_t* kt = kb + (int64_t)k0 * a.k_l;
-    const uint16_t* vt = vb + (int64_t)k0 * a.v_l;
-    const uint32_t dk = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_k[buf][wave * 64]), dv = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_v[buf][wave * 64]);
+    const uint32_t sk = dk + buf * (BK * CH * 16), sv = dv + buf * (BK * VC * 16);
 #pragma unroll
     for (int n = 0; n < kLoadsK; ++n)
-      if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH) dma16(kt, k_off[n], dk + n * kThreads * 16);
+      if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH) dma16(kt, k_off[n], sk + n * kThreads * 16);
 #pragma unroll
     for (int n = 0; n < kLoadsV; ++n)
-      if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC) dma16(vt, v_off[n], dv + n * kThreads * 16);
+      if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC) dma16(vt, v_off[n], sv + n * kThreads * 16);
+    kt += kt_step;
+    vt += vt_step;
   };
 
   f32x16 o[DT] = {};
@@ -330,33 +368,109 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_kernel(const AttnArg
   }
 
   l += __shfl_xor(l, 32);
-  const float inv = empty ? 0.f : 1.f / l;
-  bool bad = false;
   uint16_t* orow = a.out + b * a.o_b + (int64_t)pos * a.o_l + head * a.o_h;
+  float* prow = partial + (wave * kWaveRows + (lane & 31)) * (a.dim + 4);
+  const bool nothing = lo_s >= hi_s;
+  const float inv = partial ? 1.f : 1.f / l;
+  bool bad = false;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = d * 32 + e * 8 + half * 4;
-      if (live && c < a.dim) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float y = o[d][e * 4 + i] * inv;
-          x[i] = empty ? 0.f : y;
-          bad |= !empty && !(fabsf(y) < INFINITY);
-        }
-        *reinterpret_cast<u32x2*>(orow + c) = u32x2{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
-      }
+    for (int e = 0; e < 16; ++e) {
+      o[d][e] = nothing ? 0.f : o[d][e] * inv;
+      if (d * 32 + e / 4 * 8 < a.dim) bad |= !(fabsf(o[d][e]) < INFINITY);
     }
+  bad &= live;
+  // columns 32 d + 8 e + 4 half + 0..3 of this lane's row
+  if (!partial) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d * 32 + e * 8 < a.dim && live)
+          *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = u32x2{pack2<BF16>(o[d][e * 4], o[d][e * 4 + 1]), pack2<BF16>(o[d][e * 4 + 2], o[d][e * 4 + 3])};
+  } else {
+    if (live && half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d * 32 + e * 8 < a.dim && live && !nothing)
+          *reinterpret_cast<f32x4*>(prow + d * 32 + e * 8 + half * 4) = f32x4{o[d][e * 4], o[d][e * 4 + 1], o[d][e * 4 + 2], o[d][e * 4 + 3]};
+  }
   uint64_t again = __ballot(bad);
   again = (again | again >> 32) & 0xffffffffu;
   while (again) {
     const int src = __builtin_ctzll(again);
     again &= again - 1;
-    const int pos2 = __shfl(pos, src), head2 = __shfl(head, src), lo2 = __shfl(lo, src), hi2 = __shfl(hi, src);
-    exact_row<BF16, CAP>(a, a.q + b * a.q_b + (int64_t)pos2 * a.q_l + head2 * a.q_h, kb, vb, lo2, hi2, a.out + b * a.o_b + (int64_t)pos2 * a.o_l + head2 * a.o_h);
+    const int pos2 = __shfl(pos, src), head2 = __shfl(head, src), lo2 = __shfl(lo_s, src), hi2 = __shfl(hi_s, src);
+    exact_row<BF16, CAP>(a, a.q + b * a.q_b + (int64_t)pos2 * a.q_l + head2 * a.q_h, kb, vb, lo2, hi2, a.out + b * a.o_b + (int64_t)pos2 * a.o_l + head2 * a.o_h,
+                         partial ? partial + (wave * kWaveRows + src) * (a.dim + 4) : nullptr);
   }
+}
+
+// Joins the runs of keys of the cut tiles: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A wave's lanes take the runs' weights first, so
+// that the loads of the sums do not wait for one another; W waves share a row (every W-th run each), added up in their order.
+template <bool BF16, int W>
+__global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
+  constexpr int kRows = 4 / W;  // of a block
+  __shared__ f32x4 lds_o[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t all = (int64_t)a.rows * a.group;
+  const int stored = (int)min((int64_t)a.block_rows, all), blocks = (stored + kRows - 1) / kRows;
+  const int in_tile = (int)(blockIdx.x % blocks) * kRows + wave / W, cut = blockIdx.x / blocks;
+  int id = a.full + cut;
+  const int tile = a.tiles - 1 - id % a.tiles;
+  id /= a.tiles;
+  const int hk = id % a.kv_heads, b = id / a.kv_heads;
+  const int64_t r = (int64_t)tile * a.block_rows + in_tile;
+  const bool live = in_tile < stored && r < all;  // of the whole group of W waves
+  const int64_t step = (int64_t)stored * (a.dim + 4);
+  const float* src = a.partial + (int64_t)cut * a.splits * step + (int64_t)(live ? in_tile : 0) * (a.dim + 4);
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {};
+  if (live) {
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, src[s * step + a.dim]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+      float w = 0.f;  // of run s0 + lane; 0 where the row sees nothing of it (its sums were never written)
+      if (s0 + lane < a.splits) {
+        const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + a.dim);
+        if (ml.y != 0.f) w = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+        l = __builtin_fmaf(ml.y, w, l);
+      }
+      const int n = min(64, a.splits - s0);
+#pragma unroll 8
+      for (int i = wave % W; i < n; i += W) {
+        const float wi = __shfl(w, i);
+        const f32x4 part = lane * 4 < a.dim ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = wi == 0.f ? o[e] : __builtin_fmaf(part[e], wi, o[e]);
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+  }
+  if constexpr (W > 1) {
+    lds_o[wave][lane] = o;
+    __syncthreads();
+    if (wave % W) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) o += lds_o[wave + i][lane];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (live && lane * 4 < a.dim) {
+    const int64_t pos = r / a.group, head = hk * a.group + r % a.group;
+    *reinterpret_cast<u32x2*>(a.out + b * a.o_b + pos * a.o_l + head * a.o_h + lane * 4) =
+        u32x2{pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv)};
+  }
+}
+
+template <bool BF16>
+void launch_join(const AttnArgs& a, int64_t cut, int64_t stored, hipStream_t s) {
+  if (a.splits >= 16) hipLaunchKernelGGL((join_kernel<BF16, 4>), dim3((unsigned)(cut * stored)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<BF16, 1>), dim3((unsigned)(cut * ((stored + 3) / 4))), dim3(256), 0, s, a);
 }
 
 // Zero keys: every row is empty.
@@ -364,22 +478,64 @@ __global__ void zero_rows_kernel(uint32_t* out, int64_t words) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) out[i] = 0;
 }
 
+// How the tiles of a call are dealt out.  A card takes waves_per_simd waves a SIMD at once; the tiles of the last, partly filled round are cut into
+// runs of keys, as many as fill it, where what that saves (a tile takes about kTileUs per tile of keys in a filled CU) is more than writing,
+// reading and joining the runs' 32-bit sums costs (kJoinUs for the launch, kJoinBytesPerUs).
+struct Plan {
+  int64_t blocks, full, cut, splits, bytes;
+};
+constexpr double kTileUs = 2.3, kJoinUs = 4.0, kJoinBytesPerUs = 4e6;
+
+Plan plan(int64_t batch, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, int64_t cus) {
+  const int kc = built_kc((int)dim);
+  const int64_t all = rows * (heads / kv_heads), slots = cus * waves_per_simd(kc) * 4 / block_waves(kc);
+  Plan p = {};
+  p.blocks = (all + block_rows(kc) - 1) / block_rows(kc) * kv_heads * batch;
+  p.full = p.blocks / slots * slots;
+  p.cut = p.blocks - p.full;
+  p.splits = 1;
+  if (p.cut == 0) return p;
+  const int64_t key_tiles = (keys + tile_keys(kc) - 1) / tile_keys(kc);
+  const int64_t piece = std::min<int64_t>(block_rows(kc), all) * (dim + 4) * 4;
+  // t(n) = key_tiles / n * kTileUs + kJoinUs + n * moved: least at n = sqrt(key_tiles * kTileUs / moved), then evened out to whole tiles
+  const double moved = 2.0 * p.cut * piece / kJoinBytesPerUs;
+  int64_t n = (int64_t)std::sqrt(key_tiles * kTileUs / moved);
+  n = std::min<int64_t>(n, std::min<int64_t>(slots / p.cut, key_tiles));
+  if (n < 2) return p;
+  const int64_t share = (key_tiles + n - 1) / n;
+  n = (key_tiles + share - 1) / share;
+  if (share * kTileUs + kJoinUs + n * moved < key_tiles * kTileUs) p.splits = n;
+  if (p.splits > 1) p.bytes = p.cut * p.splits * piece;
+  return p;
+}
+
+int cu_count(int device) {
+  static std::atomic<int> known[64];
+  if (device < 0 || device >= 64) return 256;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1) n = 256;
+    known[device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <bool BF16, int KC, bool CAP>
 void launch_attention(const AttnArgs& a, int64_t blocks, hipStream_t s) {
-  constexpr int BK = KC > 8 ? 32 : 64;
-  hipLaunchKernelGGL((attention_kernel<BF16, KC, BK, CAP>), dim3((unsigned)blocks), dim3(kWaves * 64), 0, s, a);
+  hipLaunchKernelGGL((attention_kernel<BF16, KC, CAP>), dim3((unsigned)blocks), dim3(block_waves(KC) * 64), 0, s, a);
 }
 
 template <bool BF16, bool CAP>
 void dispatch_dim(const AttnArgs& a, int64_t blocks, hipStream_t s) {
-  const int kc = (a.dim + 15) / 16;
-  if (kc <= 2) launch_attention<BF16, 2, CAP>(a, blocks, s);
-  else if (kc <= 4) launch_attention<BF16, 4, CAP>(a, blocks, s);
-  else if (kc == 5) launch_attention<BF16, 5, CAP>(a, blocks, s);
-  else if (kc == 6) launch_attention<BF16, 6, CAP>(a, blocks, s);
-  else if (kc <= 8) launch_attention<BF16, 8, CAP>(a, blocks, s);
-  else if (kc <= 12) launch_attention<BF16, 12, CAP>(a, blocks, s);
-  else launch_attention<BF16, 16, CAP>(a, blocks, s);
+  switch (built_kc(a.dim)) {
+    case 2: return launch_attention<BF16, 2, CAP>(a, blocks, s);
+    case 4: return launch_attention<BF16, 4, CAP>(a, blocks, s);
+    case 5: return launch_attention<BF16, 5, CAP>(a, blocks, s);
+    case 6: return launch_attention<BF16, 6, CAP>(a, blocks, s);
+    case 8: return launch_attention<BF16, 8, CAP>(a, blocks, s);
+    case 12: return launch_attention<BF16, 12, CAP>(a, blocks, s);
+    default: return launch_attention<BF16, 16, CAP>(a, blocks, s);
+  }
 }
 
 // ---------------------------------------------------------------- key ranges
@@ -474,13 +630,21 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   } else {
     a.qk = p->scale * kLog2e;
   }
-  const int64_t tiles = ((int64_t)p->rows * a.group + kBlockRows - 1) / kBlockRows;
-  const int64_t blocks = tiles * p->kv_heads * p->batch;
-  if (tiles > 0x7fffffff || blocks > 0x7fffffff) {
+  const int64_t tall = (int64_t)p->rows * a.group;  // rows of one K/V head
+  const Plan pl = plan(p->batch, p->rows, p->keys, p->heads, p->kv_heads, p->dim, cu_count(device));
+  const int64_t blocks = pl.full + pl.cut * pl.splits;
+  if (pl.blocks > 0x7fffffff || blocks > 0x7fffffff) {
     set_error("mv_enc_attention: too many rows for one launch");
     return MV_ERR_INVALID;
   }
-  a.tiles = (int32_t)tiles;
+  if (pl.bytes > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 15) || p->workspace_bytes < pl.bytes)) {
+    set_error("mv_enc_attention: needs a 16-byte aligned workspace of %lld bytes (mv_enc_attention_workspace_bytes)", (long long)pl.bytes);
+    return MV_ERR_INVALID;
+  }
+  a.block_rows = block_rows(built_kc(p->dim));
+  a.tiles = (int32_t)((tall + a.block_rows - 1) / a.block_rows);
+  a.full = (int32_t)pl.full, a.splits = (int32_t)pl.splits;
+  a.partial = reinterpret_cast<float*>(p->workspace);
   DeviceGuard g(device);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (p->keys == 0) {
@@ -494,7 +658,20 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
     else dispatch_dim<false, false>(a, blocks, s);
   }
   MV_HIP(hipGetLastError());
+  if (p->keys > 0 && pl.splits > 1) {
+    if (p->dtype == MV_BF16) launch_join<true>(a, pl.cut, std::min<int64_t>(tall, a.block_rows), s);
+    else launch_join<false>(a, pl.cut, std::min<int64_t>(tall, a.block_rows), s);
+    MV_HIP(hipGetLastError());
+  }
   return MV_OK;
+}
+
+int64_t mv_enc_attention_workspace_bytes(int device, int32_t batch, int32_t rows, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim) {
+  if (batch < 0 || rows < 0 || keys < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 256 || dim % 8) {
+    set_error("mv_enc_attention_workspace_bytes: bad sizes");
+    return MV_ERR_INVALID;
+  }
+  return plan(batch, rows, keys, heads, kv_heads, dim, cu_count(device)).bytes;
 }
 
 int mv_enc_padded_ranges(int device, const int32_t* d_starts, int64_t starts_stride, const int32_t* d_ends, int64_t ends_stride, const int32_t* d_prefixes,

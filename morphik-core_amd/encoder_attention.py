@@ -19,6 +19,7 @@ are refused.  There is no CPU path: tensors off the GPU are refused.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
 from typing import Any, Optional, Sequence, Tuple
@@ -72,7 +73,8 @@ def _device_index(torch, what: str, *tensors: Any) -> int:
 
 
 def _stream(torch, index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without the Stream object around it (1 us less)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _heads4(t: Any, what: str, name: str) -> Any:
@@ -356,6 +358,14 @@ def ranges_from_mask(mask: Any) -> Tuple[Any, Any]:
 
 
 # --------------------------------------------------------------------------- attention
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(index: int, *sizes: int) -> int:
+    n = _lib.lib().mv_enc_attention_workspace_bytes(index, *sizes)
+    if n < 0:
+        _lib.check(int(n))
+    return int(n)
+
+
 def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, scale: Optional[float] = None, softcap: float = 0.0) -> Any:
     """Softmax attention of q [batch, rows, heads, dim] over k, v [batch, keys, kv_heads, dim] (or [rows, heads, dim] of packed documents), heads
     a multiple of kv_heads.  key_ranges int32 [batch or 1, rows, 2]: row i sees the keys [lo, hi), cut to what there is; an empty range gives
@@ -405,6 +415,8 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, scale: Optional
         ranges = ranges_batch = 0
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if batch and rows:
-        packed = _PACK_ATTN.pack(*pointers, out.data_ptr(), ranges, *strides, ranges_batch, code, batch, rows, keys, heads, kv_heads, dim, scale, softcap)
+        need = _workspace_bytes(index, batch, rows, keys, heads, kv_heads, dim)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # torch's own reuse rules keep it this call's on this stream
+        packed = _PACK_ATTN.pack(*pointers, out.data_ptr(), ranges, *strides, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, scale, softcap)
         _lib.check(_lib.lib().mv_enc_attention(index, packed, _stream(torch, index)))
     return out if len(shape) == 4 else out.view(shape)

@@ -494,7 +494,8 @@ typedef struct mv_rotary {
 MV_API int mv_enc_rotary(int device, const mv_rotary* p, void* stream);
 
 /*   mv_enc_attention  out[b][i][h] = softmax_j(scale * q[b][i][h] . k[b][j][h / (heads / kv_heads)]) v[b][j][...] over the keys
- *                  ranges[b][i][0] <= j < ranges[b][i][1] (cut to 0 .. keys; an empty range gives zeros; ranges NULL: every key).
+ *                  ranges[b][i][0] <= j < ranges[b][i][1] (cut to 0 .. keys; an empty range gives zeros; ranges NULL: every key, or
+ *                  with causal != 0 those up to the row itself, the last row standing at the last key).
  *                  softcap c > 0: scores become c * tanh(score / c) first.  What keys outside a row's range hold does not reach the row,
  *                  NaN and infinity included.  dtype MV_BF16 or MV_F16; dim a multiple of 8 up to 256; pointers 16-byte aligned (ranges: 8),
  *                  strides multiples of 8 (ranges: 2, 0 = one for all); out contiguous [batch][rows][heads][dim].  Sums and softmax statistics
@@ -507,7 +508,7 @@ typedef struct mv_attn {
   int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head, ranges_batch;
   void* workspace; /* scratch for this call alone (16-byte aligned), may be NULL where mv_enc_attention_workspace_bytes says 0 */
   int64_t workspace_bytes;
-  int32_t dtype, batch, rows, keys, heads, kv_heads, dim;
+  int32_t dtype, batch, rows, keys, heads, kv_heads, dim, causal;
   float scale, softcap;
 } mv_attn;
 MV_API int64_t mv_enc_attention_workspace_bytes(int device, int32_t batch, int32_t rows, int32_t keys, int32_t heads, int32_t kv_heads, int32_t dim);

@@ -92,7 +92,7 @@ class AttnC(C.Structure):
         [(n, C.c_void_p) for n in ("q", "k", "v", "out", "ranges")]
         + [(n, C.c_int64) for n in ("q_batch", "q_row", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row", "v_head", "ranges_batch")]
         + [("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
-        + [(n, C.c_int32) for n in ("dtype", "batch", "rows", "keys", "heads", "kv_heads", "dim")] + [("scale", C.c_float), ("softcap", C.c_float)]
+        + [(n, C.c_int32) for n in ("dtype", "batch", "rows", "keys", "heads", "kv_heads", "dim", "causal")] + [("scale", C.c_float), ("softcap", C.c_float)]
     )
 
 

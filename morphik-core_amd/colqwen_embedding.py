@@ -91,7 +91,7 @@ def build_random_colqwen2(preset: str, tokenizer_ids: Dict[str, int], device, dt
 
 class MI355XColQwen2EmbeddingModel(BaseEmbeddingModel):
     def __init__(self, model_name_or_path: Optional[str] = None, model: Any = None, processor: Any = None, device: Optional[str] = None,
-                 batch_size: int = 8, fused_ops: Optional[bool] = None):
+                 batch_size: int = 8, fused_ops: Optional[bool] = None, fused_attention: Optional[bool] = None):
         import torch
 
         self.torch = torch
@@ -118,6 +118,13 @@ class MI355XColQwen2EmbeddingModel(BaseEmbeddingModel):
 
             if fused_ops or encoder_ops.enabled_by_env():
                 self.fused_ops = encoder_ops.patch_encoder(self.model)
+        # rotary positions and attention as HIP kernels (encoder_attention.py): on request, or where MV_ENCODER_FUSED_ATTENTION=1
+        self.fused_attention = {"rotary": 0, "decoder": 0, "packed": 0}
+        if self.device.type == "cuda" and fused_attention is not False:
+            from . import encoder_attention
+
+            if fused_attention or encoder_attention.enabled_by_env():
+                self.fused_attention = encoder_attention.patch_attention(self.model)
 
     # ------------------------------------------------------------------ forward
     def _forward(self, batch) -> Tuple[Any, Any]:

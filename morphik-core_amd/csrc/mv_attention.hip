@@ -53,7 +53,7 @@ struct AttnArgs {
   uint16_t* out;
   const int32_t* ranges;  // [batch or 1][rows][2] or null: every row sees every key
   int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, o_b, o_l, o_h, range_b;  // strides in elements
-  int32_t rows, keys, kv_heads, group, dim, tiles, block_rows;  // tiles: blocks of block_rows over rows * group
+  int32_t rows, keys, kv_heads, group, dim, tiles, block_rows, causal;  // tiles: blocks of block_rows over rows * group
   int32_t full, splits;  // blocks [0, full) take a tile each; the tiles behind them are cut into `splits` runs of keys, one block each
   float* partial;        // of those: [tile - full][split][rows of a tile] x (dim sums, maximum, sum of weights, 2 unused)
   float qk;    // scale * log2(e); with a cap: scale / cap * 2 log2(e)
@@ -207,6 +207,8 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     const int2 rg = *reinterpret_cast<const int2*>(a.ranges + b * a.range_b + (int64_t)pos * 2);
     lo = max(rg.x, 0);
     hi = min(rg.y, a.keys);
+  } else if (live && a.causal) {
+    hi = (int)min((int64_t)pos + 1 + a.keys - a.rows, (int64_t)a.keys);
   }
   if (lo >= hi) lo = hi = 0;
   const bool empty = lo == hi;
@@ -623,7 +625,7 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   a.k_b = p->k_batch, a.k_l = p->k_row, a.k_h = p->k_head;
   a.v_b = p->v_batch, a.v_l = p->v_row, a.v_h = p->v_head;
   a.o_h = p->dim, a.o_l = (int64_t)p->heads * p->dim, a.o_b = a.o_l * p->rows;
-  a.rows = p->rows, a.keys = p->keys, a.kv_heads = p->kv_heads, a.group = p->heads / p->kv_heads, a.dim = p->dim;
+  a.rows = p->rows, a.keys = p->keys, a.kv_heads = p->kv_heads, a.group = p->heads / p->kv_heads, a.dim = p->dim, a.causal = p->causal && !p->ranges;
   if (p->softcap > 0.f) {
     a.qk = (float)((double)p->scale / p->softcap * 2.0 * 1.4426950408889634);
     a.cap = p->softcap * kLog2e;

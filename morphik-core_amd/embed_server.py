@@ -86,6 +86,8 @@ def main(argv: Optional[List[str]] = None) -> None:
     ap.add_argument("--preset", default="colpali-v1.2")
     ap.add_argument("--device", default=None)
     ap.add_argument("--batch-size", type=int, default=8)
+    ap.add_argument("--fused-attention", action="store_true", default=None,
+                    help="rotary positions and attention of the encoder as HIP kernels (default: where MV_ENCODER_FUSED_ATTENTION=1)")
     a = ap.parse_args(argv)
     import uvicorn
 
@@ -94,11 +96,13 @@ def main(argv: Optional[List[str]] = None) -> None:
             raise SystemExit("embed_server: --family colqwen2 needs --model <checkpoint directory> (its processor ships with the checkpoint)")
         from .colqwen_embedding import MI355XColQwen2EmbeddingModel
 
-        emb: Any = MI355XColQwen2EmbeddingModel(model_name_or_path=a.model, device=a.device, batch_size=a.batch_size)
+        emb: Any = MI355XColQwen2EmbeddingModel(model_name_or_path=a.model, device=a.device, batch_size=a.batch_size,
+                                                fused_attention=a.fused_attention)
     else:
         from .embedding import MI355XColpaliEmbeddingModel
 
-        emb = MI355XColpaliEmbeddingModel(model_name_or_path=a.model, preset=a.preset, device=a.device, batch_size=a.batch_size)
+        emb = MI355XColpaliEmbeddingModel(model_name_or_path=a.model, preset=a.preset, device=a.device, batch_size=a.batch_size,
+                                                fused_attention=a.fused_attention)
     uvicorn.run(create_app(emb, os.environ.get("MORPHIK_EMBEDDING_API_KEY")), host=a.host, port=a.port, log_level="info")
 
 

@@ -21,8 +21,10 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import os
 import struct
-from typing import Any, Optional, Sequence, Tuple
+import types
+from typing import Any, Dict, Optional, Sequence, Tuple
 
 from . import _lib
 
@@ -150,47 +152,49 @@ class RotaryTable:
 
 
 def _rotary_operands(torch, what, q, k, in_place):
-    """-> (q and k as [batch, rows, heads, dim] or None, outputs in that form, outputs as the caller shaped them)"""
-    first = q if q is not None else k
-    if first is None:
+    """-> (q, k, their outputs as [batch, rows, heads, dim] or None, outputs as the caller shaped them)"""
+    if q is None and k is None:
         raise ValueError(f"{what}: neither q nor k")
-    ins, outs, shaped = [], [], []
-    for n, t in (("q", q), ("k", k)):
-        if t is None:
-            ins.append(None), outs.append(None), shaped.append(None)
-            continue
-        x = _heads4(t, what, n)
-        st = x.stride()
-        if st[3] != 1 and x.shape[3] > 1 and x.numel():
-            raise ValueError(f"{what}: the elements of a head of {n} must lie next to each other")
-        if in_place:
-            if _overlaps(x):
-                raise ValueError(f"{what}: {n} cannot be turned in place, its heads or rows share memory")
-            out = x
-        else:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        ins.append(x), outs.append(out), shaped.append(t if in_place else out if x is t else out.view(t.shape))
-    if q is not None and k is not None:
-        a, b = ins[0].shape, ins[1].shape
-        if q.dtype is not k.dtype or a[:2] != b[:2] or a[3] != b[3]:
-            raise ValueError(f"{what}: q and k differ in type, batch, rows or head width ({tuple(a)} {q.dtype}, {tuple(b)} {k.dtype})")
-        if in_place and _share_memory(*ins):
+    x, xo, x_shaped = _rotary_operand(torch, what, "q", q, in_place)
+    y, yo, y_shaped = _rotary_operand(torch, what, "k", k, in_place)
+    if x is not None and y is not None:
+        a, b = x.shape, y.shape
+        if x.dtype is not y.dtype or a[0] != b[0] or a[1] != b[1] or a[3] != b[3]:
+            raise ValueError(f"{what}: q and k differ in type, batch, rows or head width ({tuple(a)} {x.dtype}, {tuple(b)} {y.dtype})")
+        if in_place and _share_memory(x, y):
             raise ValueError(f"{what}: q and k cannot be turned in place, they share memory")
-    return ins, outs, tuple(shaped)
+    return x, y, xo, yo, (x_shaped, y_shaped)
+
+
+def _rotary_operand(torch, what, name, t, in_place):
+    if t is None:
+        return None, None, None
+    x = _heads4(t, what, name)
+    if x.stride(3) != 1 and x.shape[3] > 1 and x.numel():
+        raise ValueError(f"{what}: the elements of a head of {name} must lie next to each other")
+    if not in_place:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        return x, out, out if x is t else out.view(t.shape)
+    if _overlaps(x):
+        raise ValueError(f"{what}: {name} cannot be turned in place, its heads or rows share memory")
+    return x, x, t
 
 
 _NO_STRIDES = (0, 0, 0)
 
 
-def _launch_rotary(torch, what, ins, outs, first, index, pos, pos_strides, freq, axis, cos, sin, table_strides, scale, adjacent, pairs):
-    (q, k), (qo, ko) = ins, outs
-    batch, rows, _, dim = first.shape
-    code = _dtype_code(torch, first.dtype, what, fp32=True)
-    packed = _PACK_ROTARY.pack(
-        *(0 if t is None else t.data_ptr() for t in (q, k, qo, ko)),
-        *(st for t in (q, k, qo, ko) for st in (_NO_STRIDES if t is None else t.stride()[:3])),
-        0 if pos is None else pos.data_ptr(), *pos_strides, freq, axis, cos, sin, *table_strides, scale, code,
-        int(pos is not None and pos.dtype is torch.int64), adjacent, batch, rows, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], dim, pairs)
+def _launch_rotary(torch, what, q, k, qo, ko, index, code, positions, pos_strides, freq, axis, cos, sin, table_strides, scale, wide_positions, adjacent, pairs):
+    batch, rows, heads, dim = q.shape if q is not None else k.shape
+    if q is None:
+        heads, at_q, at_qo, st_q, st_qo = 0, 0, 0, _NO_STRIDES, _NO_STRIDES
+    else:
+        at_q, at_qo, st_q, st_qo = q.data_ptr(), qo.data_ptr(), q.stride()[:3], qo.stride()[:3]
+    if k is None:
+        kv_heads, at_k, at_ko, st_k, st_ko = 0, 0, 0, _NO_STRIDES, _NO_STRIDES
+    else:
+        kv_heads, at_k, at_ko, st_k, st_ko = k.shape[2], k.data_ptr(), ko.data_ptr(), k.stride()[:3], ko.stride()[:3]
+    packed = _PACK_ROTARY.pack(at_q, at_k, at_qo, at_ko, *st_q, *st_k, *st_qo, *st_ko, positions, *pos_strides, freq, axis, cos, sin, *table_strides, scale, code,
+                               wide_positions, adjacent, batch, rows, heads, kv_heads, dim, pairs)
     _lib.check(_lib.lib().mv_enc_rotary(index, packed, _stream(torch, index)))
 
 
@@ -237,9 +241,9 @@ def rotary(q: Any, k: Any, positions: Any, table: RotaryTable, *, in_place: bool
     what = "rotary"
     if not isinstance(table, RotaryTable):
         raise ValueError(f"{what}: table must be a RotaryTable")
-    ins, outs, shaped = _rotary_operands(torch, what, q, k, in_place)
-    first = ins[0] if ins[0] is not None else ins[1]
-    _dtype_code(torch, first.dtype, what, fp32=True)
+    x, y, xo, yo, shaped = _rotary_operands(torch, what, q, k, in_place)
+    first = x if x is not None else y
+    code = _dtype_code(torch, first.dtype, what, fp32=True)
     batch, rows, _, dim = first.shape
     if dim != table.head_dim:
         raise ValueError(f"{what}: heads of {dim}, the table is for {table.head_dim}")
@@ -256,10 +260,10 @@ def rotary(q: Any, k: Any, positions: Any, table: RotaryTable, *, in_place: bool
         raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit {batch} x {rows} rows")
     if pos.shape[0] < table.axes:
         raise ValueError(f"{what}: positions have {pos.shape[0]} axes, the table needs {table.axes}")
-    index = _device_index(torch, what, first, *([ins[1]] if ins[1] is not None else []), pos, table.inv_freq)
+    index = _device_index(torch, what, first, pos, table.inv_freq, first if y is None else y)
     st = pos.stride()
-    _launch_rotary(torch, what, ins, outs, first, index, pos, (st[0], st[1] if pos.shape[1] == batch else 0, st[2]), table.inv_freq.data_ptr(),
-                   table.axis.data_ptr(), 0, 0, _NO_STRIDES, table.scale, int(table.pairing == "adjacent"), table.pairs)
+    _launch_rotary(torch, what, x, y, xo, yo, index, code, pos.data_ptr(), (st[0], st[1] if pos.shape[1] == batch else 0, st[2]), table.inv_freq.data_ptr(),
+                   table.axis.data_ptr(), 0, 0, _NO_STRIDES, table.scale, int(pos.dtype is torch.int64), int(table.pairing == "adjacent"), table.pairs)
     return shaped
 
 
@@ -270,9 +274,9 @@ def rotary_tables(q: Any, k: Any, cos: Any, sin: Any, *, pairing: str = "halves"
     what = "rotary_tables"
     if pairing not in _PAIRINGS:
         raise ValueError(f"{what}: pairing {pairing!r} (one of {_PAIRINGS})")
-    ins, outs, shaped = _rotary_operands(torch, what, q, k, in_place)
-    first = ins[0] if ins[0] is not None else ins[1]
-    _dtype_code(torch, first.dtype, what, fp32=True)
+    x, y, xo, yo, shaped = _rotary_operands(torch, what, q, k, in_place)
+    first = x if x is not None else y
+    code = _dtype_code(torch, first.dtype, what, fp32=True)
     batch, rows, _, dim = first.shape
     if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError(f"{what}: cos and sin must be float32")
@@ -282,10 +286,10 @@ def rotary_tables(q: Any, k: Any, cos: Any, sin: Any, *, pairing: str = "halves"
         cos, sin = cos[None], sin[None]
     if cos.dim() != 3 or cos.shape[0] not in (1, batch) or cos.shape[1] != rows or not 0 < 2 * cos.shape[2] <= dim <= 4096:
         raise ValueError(f"{what}: cos of {tuple(cos.shape)} does not fit {batch} x {rows} rows of heads of {dim} (at most 4096)")
-    index = _device_index(torch, what, first, *([ins[1]] if ins[1] is not None else []), cos, sin)
+    index = _device_index(torch, what, first, cos, sin, first if y is None else y)
     st = cos.stride()
-    _launch_rotary(torch, what, ins, outs, first, index, None, _NO_STRIDES, 0, 0, cos.data_ptr(), sin.data_ptr(),
-                   (st[0] if cos.shape[0] == batch else 0, st[1], st[2]), 1.0, int(pairing == "adjacent"), cos.shape[2])
+    _launch_rotary(torch, what, x, y, xo, yo, index, code, 0, _NO_STRIDES, 0, 0, cos.data_ptr(), sin.data_ptr(),
+                   (st[0] if cos.shape[0] == batch else 0, st[1], st[2]), 1.0, 0, int(pairing == "adjacent"), cos.shape[2])
     return shaped
 
 
@@ -366,10 +370,10 @@ def _workspace_bytes(index: int, *sizes: int) -> int:
     return int(n)
 
 
-def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, scale: Optional[float] = None, softcap: float = 0.0) -> Any:
+def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = False, scale: Optional[float] = None, softcap: float = 0.0) -> Any:
     """Softmax attention of q [batch, rows, heads, dim] over k, v [batch, keys, kv_heads, dim] (or [rows, heads, dim] of packed documents), heads
     a multiple of kv_heads.  key_ranges int32 [batch or 1, rows, 2]: row i sees the keys [lo, hi), cut to what there is; an empty range gives
-    zeros; None: every key.  scale defaults to dim ** -0.5; softcap c > 0 caps scores to c * tanh(score / c).  bfloat16 or float16; dim a multiple
+    zeros; None: every key, or with `causal` those up to the row itself (the last row stands at the last key).  scale defaults to dim ** -0.5; softcap c > 0 caps scores to c * tanh(score / c).  bfloat16 or float16; dim a multiple
     of 8 up to 256; any strides that are multiples of 8 with the elements of a head side by side, 16-byte aligned.
     -> new contiguous tensor of q's shape."""
     torch = _torch()
@@ -404,6 +408,8 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, scale: Optional
         pointers.append(at)
         strides += st[:3]
     if key_ranges is not None:
+        if causal:
+            raise ValueError(f"{what}: causal goes without key_ranges (padded_ranges(..., prefix=0) makes causal ones)")
         if key_ranges.dtype is not torch.int32 or key_ranges.dim() != 3 or key_ranges.shape[0] not in (1, batch) or tuple(key_ranges.shape[1:]) != (rows, 2):
             raise ValueError(f"{what}: key_ranges must be int32 [{batch} or 1, {rows}, 2], not {key_ranges.dtype} {tuple(key_ranges.shape)}")
         index = _device_index(torch, what, q, k, v, key_ranges)
@@ -413,10 +419,185 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, scale: Optional
     else:
         index = _device_index(torch, what, q, k, v)
         ranges = ranges_batch = 0
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if batch and rows:
         need = _workspace_bytes(index, batch, rows, keys, heads, kv_heads, dim)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # torch's own reuse rules keep it this call's on this stream
-        packed = _PACK_ATTN.pack(*pointers, out.data_ptr(), ranges, *strides, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, scale, softcap)
+        packed = _PACK_ATTN.pack(*pointers, out.data_ptr(), ranges, *strides, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, int(causal), scale, softcap)
         _lib.check(_lib.lib().mv_enc_attention(index, packed, _stream(torch, index)))
     return out if len(shape) == 4 else out.view(shape)
+
+
+# --------------------------------------------------------------------------- the encoders' own blocks
+_NAME = "mv_key_ranges"  # of the attention and mask functions registered with transformers
+_DECODERS = ("GemmaAttention", "Qwen2VLAttention", "Qwen2_5_VLAttention")
+_PACKED = ("VisionAttention", "Qwen2_5_VLVisionAttention")
+
+
+class _Angles(tuple):
+    """(cos, sin) as a rotary module returns them, and what they were made of: positions [axes, batch, rows] and the RotaryTable."""
+
+    positions: Any = None
+    table: Any = None
+
+
+def enabled_by_env() -> bool:
+    return os.environ.get("MV_ENCODER_FUSED_ATTENTION", "0") in ("1", "true", "yes")
+
+
+def _kernel_takes(torch, *tensors) -> bool:
+    """Inference on a GPU in a type and layout that `attention` has; anything else goes the framework's way."""
+    first = tensors[0]
+    if not first.is_cuda or torch.is_grad_enabled() or first.dtype not in (torch.bfloat16, torch.float16) or first.shape[-1] % 8 or not 8 <= first.shape[-1] <= 256:
+        return False
+    return all(t.dtype == first.dtype and t.device == first.device and t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(st % 8 for st in t.stride()[:-1])
+               for t in tensors)
+
+
+def _interface_attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, softcap=None, is_causal=None, **kwargs):
+    """transformers' attention function: query [batch, heads, rows, dim], key / value [batch, kv_heads, keys, dim] -> ([batch, rows, heads, dim], None)."""
+    torch = _torch()
+    ranges = attention_mask[:, 0] if attention_mask is not None and attention_mask.dtype == torch.int32 else None
+    causal = getattr(module, "is_causal", False) if is_causal is None else is_causal
+    causal = bool(causal) and attention_mask is None and query.shape[2] > 1
+    known = ranges is not None or attention_mask is None and not (causal and query.shape[2] != key.shape[2])
+    if known and not dropout and _kernel_takes(torch, query, key, value):
+        out = attention(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), key_ranges=ranges, causal=causal, scale=scaling, softcap=softcap or 0.0)
+        return out, None
+    from transformers import AttentionInterface
+
+    if ranges is not None:  # back to a boolean mask
+        at = torch.arange(key.shape[2], device=query.device, dtype=torch.int32)
+        attention_mask = ((at >= ranges[..., :1]) & (at < ranges[..., 1:]))[:, None]
+    return AttentionInterface()["sdpa"](module, query, key, value, attention_mask, scaling=scaling, dropout=dropout, is_causal=is_causal, **kwargs)
+
+
+def _interface_mask(*args, **kwargs):
+    """transformers' mask function: once per forward, the mask as key ranges int32 [batch, 1, rows, 2] where every row's keys are one run (causal, padded,
+    prefix and packed masks are), as the boolean mask otherwise (asking costs one wait for the GPU a forward).  None stays None: the attention function
+    goes by the module's is_causal then, as the framework's own does."""
+    from transformers import AttentionMaskInterface
+
+    torch = _torch()
+    mask = AttentionMaskInterface()["sdpa"](*args, **kwargs)
+    if mask is None or mask.dtype != torch.bool or mask.dim() != 4 or mask.shape[1] != 1 or not mask.is_cuda or torch.cuda.is_current_stream_capturing():
+        return mask
+    ranges, exact = ranges_from_mask(mask[:, 0])
+    return ranges[:, None] if bool(exact) else mask
+
+
+def _rotary_forward(self, x, position_ids, *args, **kwargs):
+    torch = _torch()
+    angles = self._mv_attn_forward(x, position_ids, *args, **kwargs)
+    if not x.is_cuda or torch.is_grad_enabled() or position_ids.dtype not in (torch.int32, torch.int64) or position_ids.dim() not in (2, 3):
+        return angles
+    table = self._mv_rotary_table
+    if table is None or table.inv_freq.device != x.device:
+        sections = self._mv_rotary_sections
+        axes = None if sections is None else [a for a, n in enumerate(sections) for _ in range(n)]
+        table = self._mv_rotary_table = RotaryTable(self.inv_freq, axes, head_dim=2 * int(self.inv_freq.shape[0]), scale=float(getattr(self, "attention_scaling", 1.0)),
+                                                    device=x.device)
+    positions = position_ids[None] if position_ids.dim() == 2 else position_ids
+    if positions.shape[0] < table.axes:
+        return angles
+    out = _Angles(angles)
+    out.positions, out.table = positions, table
+    return out
+
+
+def _decoder_forward(self, *args, **kwargs):
+    """q, k, v -> rotation in place -> attention over key ranges -> output projection; what does not fit goes through the module's own forward."""
+    torch = _torch()
+    x, mask, angles = kwargs.get("hidden_states"), kwargs.get("attention_mask"), kwargs.get("position_embeddings")
+    if (args or x is None or x.dim() != 3 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16)
+            or (mask is not None and mask.dtype != torch.int32) or not isinstance(angles, _Angles) or angles.table.head_dim != self.head_dim or self.head_dim % 8 or self.head_dim > 256):
+        return self._mv_attn_forward(*args, **kwargs)
+    batch, rows = x.shape[:2]
+    q, k, v = (proj(x).view(batch, rows, -1, self.head_dim) for proj in (self.q_proj, self.k_proj, self.v_proj))
+    q, k = rotary(q, k, angles.positions, angles.table, in_place=True)
+    cache = kwargs.get("past_key_values")
+    if cache is not None:
+        k, v = (t.transpose(1, 2) for t in cache.update(k.transpose(1, 2), v.transpose(1, 2), self.layer_idx))
+    if mask is not None:
+        out = attention(q, k, v, key_ranges=mask[:, 0], scale=self.scaling)
+    else:
+        out = attention(q, k, v, causal=self.is_causal and rows > 1, scale=self.scaling)
+    return self.o_proj(out.flatten(2)), None
+
+
+def _packed_forward(self, hidden_states, *args, **kwargs):
+    """Packed patches: fused projection -> rotation by the tower's tables, in place -> attention within each document or window -> output projection."""
+    torch = _torch()
+    x, offsets, angles = hidden_states, kwargs.get("cu_seqlens"), kwargs.get("position_embeddings")
+    dim = self.head_dim
+    if (args or x.dim() != 2 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16) or offsets is None or angles is None
+            or offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.device != x.device or angles[0].dtype != torch.float32
+            or angles[0].shape != (x.shape[0], dim) or dim % 8 or dim > 256):
+        return self._mv_attn_forward(hidden_states, *args, **kwargs)
+    q, k, v = self.qkv(x).view(x.shape[0], 3, -1, dim).unbind(1)
+    cos, sin = (t[:, : dim // 2] for t in angles)
+    q, k = rotary_tables(q, k, cos, sin, in_place=True)
+    out = attention(q, k, v, key_ranges=document_ranges(offsets, x.shape[0]), scale=self.scaling)
+    return self.proj(out.flatten(1))
+
+
+def _implementations(model: Any) -> list:
+    """(configuration, its attention function) of every part of the model."""
+    seen: Dict[int, Any] = {}
+    for mod in model.modules():
+        config = getattr(mod, "config", None)
+        if config is not None and hasattr(config, "_attn_implementation"):
+            seen.setdefault(id(config), (config, config._attn_implementation))
+    return list(seen.values())
+
+
+def patch_attention(model: Any) -> Dict[str, int]:
+    """Run the attention of a transformers encoder through this module, in place: the model's attention function becomes `attention` (with the mask
+    of a forward as key ranges), its decoder blocks rotate by positions, its packed vision blocks attend all documents and windows in one launch (the
+    framework takes them one by one).  Modules fall back to their own forward for anything the kernels do not take (not on a GPU, autograd on, another
+    type, a mask with holes).  -> modules patched per kind.  `unpatch_attention` undoes it."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+
+    counts = {"rotary": 0, "decoder": 0, "packed": 0}
+    if hasattr(model, "_mv_attn_before"):
+        return counts
+    AttentionInterface.register(_NAME, _interface_attention)
+    AttentionMaskInterface.register(_NAME, _interface_mask)
+    model._mv_attn_before = _implementations(model)
+    model.set_attn_implementation(_NAME)
+    for mod in model.modules():
+        cls, children = type(mod).__name__, {n for n, _ in mod.named_children()}
+        if cls.endswith("RotaryEmbedding") and hasattr(mod, "inv_freq") and getattr(mod, "rope_type", None) == "default":
+            config = getattr(mod, "config", None)
+            params = getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {}
+            sections = params.get("mrope_section")
+            if sections is not None and sum(sections) != mod.inv_freq.shape[0]:
+                continue
+            mod._mv_rotary_sections, mod._mv_rotary_table = sections, None
+            kind, forward = "rotary", _rotary_forward
+        elif cls in _DECODERS and children == {"q_proj", "k_proj", "v_proj", "o_proj"}:
+            kind, forward = "decoder", _decoder_forward
+        elif cls in _PACKED and children == {"qkv", "proj"}:
+            kind, forward = "packed", _packed_forward
+        else:
+            continue
+        mod._mv_attn_forward = mod.forward
+        mod.forward = types.MethodType(forward, mod)
+        counts[kind] += 1
+    return counts
+
+
+def unpatch_attention(model: Any) -> None:
+    """Give every module its own forward back and the model the attention function it had."""
+    if not hasattr(model, "_mv_attn_before"):
+        return
+    for config, name in model._mv_attn_before:  # one by one: set_attn_implementation leaves parts of a model that have been changed before
+        config._attn_implementation = name
+    del model._mv_attn_before
+    for mod in model.modules():
+        if hasattr(mod, "_mv_attn_forward"):
+            mod.forward = mod._mv_attn_forward
+            del mod._mv_attn_forward
+        for name in ("_mv_rotary_table", "_mv_rotary_sections"):
+            if hasattr(mod, name):
+                delattr(mod, name)

@@ -48,6 +48,8 @@ def test_attention_refuses_what_it_cannot_do():
     for cap in (-1.0, math.inf, math.nan):
         with pytest.raises(ValueError, match="softcap"):
             ea.attention(q, k, v, softcap=cap)
+    with pytest.raises(ValueError, match="causal goes without"):
+        ea.attention(q, k, v, causal=True, key_ranges=torch.zeros(2, 5, 2, dtype=torch.int32))
     with pytest.raises(ValueError, match="batch, rows, heads, dim"):
         ea.attention(q[0, 0], k, v)
     with pytest.raises(ValueError, match="side by side"):
@@ -258,3 +260,64 @@ def test_the_attention_kernels_keep_the_wait_states_of_their_matrix_results(tmp_
     for name in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"):
         assert name not in text
     shutil.rmtree(tmp_path, ignore_errors=True)
+
+
+def _outputs(model, batches):
+    with torch.inference_mode():
+        return [model(**b).embeddings.clone() for b in batches]
+
+
+@pytest.mark.parametrize("preset", ["colpali", "tiny", "tiny-2.5"])
+def test_patched_attention_leaves_a_model_without_a_gpu_exactly_as_it_was(preset):
+    """patch_attention on a CPU model: every rotary, decoder and packed module is found, and each falls back to its own forward (the attention function to
+    the framework's): bit-identical outputs, before, between and after; patching twice does nothing."""
+    ids = torch.tensor([[1, 5, 9, 3, 2], [1, 7, 0, 0, 0]])
+    batches = [dict(input_ids=ids, attention_mask=torch.ones_like(ids)), dict(input_ids=ids, attention_mask=(ids > 0).long())]
+    if preset == "colpali":
+        from morphik_core_amd.embedding import MI355XColpaliEmbeddingModel
+
+        emb = MI355XColpaliEmbeddingModel(preset="tiny", device="cpu", seed=3)
+        assert emb.fused_attention == {"rotary": 0, "decoder": 0, "packed": 0}  # never without a GPU
+        model, want_counts = emb.model, {"rotary": 1, "decoder": 2, "packed": 0}
+        pv = torch.rand(1, 3, 56, 56, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+        batches.append(dict(input_ids=torch.tensor([[1023] * 16 + [1, 4, 2]]), attention_mask=torch.ones(1, 19, dtype=torch.long), pixel_values=pv))
+    else:
+        import numpy as np
+
+        from morphik_core_amd.colqwen_embedding import build_random_colqwen2
+        from tests import offline_assets as oa
+
+        proc, tokens = oa.colqwen2_processor()
+        model, want_counts = build_random_colqwen2(preset, tokens, "cpu", torch.bfloat16), {"rotary": 1, "decoder": 2, "packed": 2}
+        rng = np.random.default_rng(0)
+        b = proc(images=[oa.page_image(rng, 60, 60), oa.page_image(rng, 112, 84)], return_tensors="pt")
+        batches.append({k: b[k].to(torch.bfloat16) if k == "pixel_values" else b[k] for k in ("input_ids", "attention_mask", "pixel_values", "image_grid_thw")})
+    before = [name for _, name in ea._implementations(model)]
+    want = _outputs(model, batches)
+    assert ea.patch_attention(model) == want_counts
+    assert ea.patch_attention(model) == {"rotary": 0, "decoder": 0, "packed": 0}
+    assert {name for _, name in ea._implementations(model)} == {"mv_key_ranges"}
+    assert all(torch.equal(a, b) for a, b in zip(_outputs(model, batches), want))
+    ea.unpatch_attention(model)
+    assert [name for _, name in ea._implementations(model)] == before and not any(hasattr(m, "_mv_attn_forward") or hasattr(m, "_mv_rotary_table") for m in model.modules())
+    assert all(torch.equal(a, b) for a, b in zip(_outputs(model, batches), want))
+    ea.unpatch_attention(model)
+
+
+def test_the_attention_function_turns_ranges_back_into_a_mask_where_the_kernel_does_not_apply():
+    class Module(torch.nn.Module):
+        is_causal = True
+        num_key_value_groups = 2
+
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(2, h, 5, 16, generator=g) for h in (4, 2, 2))
+    r = torch.tensor([[[0, 1], [0, 2], [0, 3], [1, 4], [0, 5]], [[2, 5], [2, 3], [0, 5], [0, 5], [4, 5]]], dtype=torch.int32)
+    m = torch.zeros(2, 1, 5, 5, dtype=torch.bool)
+    for b in range(2):
+        for i, (lo, hi) in enumerate(r[b].tolist()):
+            m[b, 0, i, lo:hi] = True
+    from transformers import AttentionInterface
+
+    want = AttentionInterface()["sdpa"](Module(), q, k, v, m, scaling=0.25, dropout=0.0)[0]
+    got = ea._interface_attention(Module(), q, k, v, r[:, None], scaling=0.25)[0]
+    assert torch.equal(got, want)

@@ -469,3 +469,113 @@ def test_refusals_on_the_device(ea):
             ea.rotary(q.clone().requires_grad_(), k, torch.zeros(4, dtype=torch.int64, device="cuda"), ea.RotaryTable.with_sections(16, [8]))
     with torch.no_grad():
         ea.attention(q.clone().requires_grad_(), k, v)
+
+
+@pytest.mark.parametrize("rows,keys", [(1, 1), (77, 77), (5, 300), (300, 5), (200, 450)])
+def test_causal_without_ranges(ea, rows, keys):
+    g = gen(rows + keys)
+    q, k, v = (make(g, 2, n, h, 72, DT["bf16"], "split") for n, h in ((rows, 6), (keys, 2), (keys, 2)))
+    full = torch.full((2,), keys, dtype=torch.int32, device="cuda")
+    at = torch.arange(rows, device="cuda", dtype=torch.int32) + keys - rows
+    r = torch.stack([torch.zeros_like(at), (at + 1).clamp_min(0)], -1)[None]
+    got = ea.attention(q, k, v, causal=True)
+    check(got, *oracle(q, k, v, r))
+    if rows <= keys:
+        assert torch.equal(got, ea.attention(q, k, v, key_ranges=ea.padded_ranges(torch.zeros_like(full), full, rows, prefix=0, row_offset=keys - rows)))
+
+
+# --------------------------------------------------------------------------- the encoders
+def _encoder(kind):
+    """A small random model of an encoder family with heads that the kernels take, in bf16 on the GPU, and batches for it: text of one length, padded
+    text, images."""
+    import numpy as np
+
+    from tests import offline_assets as oa
+
+    g = torch.Generator().manual_seed(7)
+    if kind == "colpali":
+        from transformers import ColPaliConfig, ColPaliForRetrieval, PaliGemmaConfig
+        from transformers.models.gemma import GemmaConfig
+        from transformers.models.siglip import SiglipVisionConfig
+
+        vis = SiglipVisionConfig(vision_use_head=False, hidden_size=144, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2, image_size=56, patch_size=14)
+        txt = GemmaConfig(hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=1, head_dim=256, vocab_size=300)
+        cfg = ColPaliConfig(vlm_config=PaliGemmaConfig(vision_config=vis, text_config=txt, image_token_index=299, projection_dim=256, hidden_size=256, vocab_size=300), embedding_dim=128)
+        torch.manual_seed(5)
+        model = ColPaliForRetrieval(cfg).to(torch.bfloat16).cuda().eval()
+        images = dict(input_ids=torch.tensor([[299] * 16 + [1, 4, 2]] * 2), attention_mask=torch.ones(2, 19, dtype=torch.long), pixel_values=torch.rand(2, 3, 56, 56, generator=g).to(torch.bfloat16))
+    else:
+        from morphik_core_amd import colqwen_embedding as cq
+
+        base = cq.PRESETS["tiny-2.5" if kind == "colqwen2.5" else "tiny"]
+        widths = dict(hidden_size=160, out_hidden_size=256) if kind == "colqwen2.5" else dict(embed_dim=160, hidden_size=256)
+        cq.PRESETS["_test"] = dict(base, vision={**base["vision"], **widths, "num_heads": 2},
+                                   text={**base["text"], "hidden_size": 256, "num_attention_heads": 2, "num_key_value_heads": 1})
+        proc, tokens = oa.colqwen2_processor()
+        try:
+            model = cq.build_random_colqwen2("_test", tokens, "cuda", torch.bfloat16)
+        finally:
+            del cq.PRESETS["_test"]
+        rng = np.random.default_rng(0)
+        b = proc(images=[oa.page_image(rng, 60, 60), oa.page_image(rng, 112, 84), oa.page_image(rng, 200, 140)], return_tensors="pt")
+        images = {k: b[k].to(torch.bfloat16) if k == "pixel_values" else b[k] for k in ("input_ids", "attention_mask", "pixel_values", "image_grid_thw")}
+    ids = torch.randint(1, 50, (3, 21), generator=g)
+    padded = torch.ones_like(ids)
+    padded[1, 13:] = 0
+    padded[2, 1:] = 0
+    batches = [dict(input_ids=ids, attention_mask=torch.ones_like(ids)), dict(input_ids=ids, attention_mask=padded), images]
+    return model, [{k: v.cuda() for k, v in b.items()} for b in batches]
+
+
+@pytest.mark.parametrize("kind", ["colpali", "colqwen2", "colqwen2.5"])
+def test_encoders_with_patched_attention_embed_as_before(ea, kind, monkeypatch):
+    """The patched model against itself in float32: no further off than the unpatched bf16 model is (its own roundings set the scale: half as far again,
+    and a floor of four bf16 steps of a unit vector's rows), with the kernels running and nothing falling back; then unpatched, its own results again."""
+    import copy
+
+    model, batches = _encoder(kind)
+    wide = copy.deepcopy(model).float()
+
+    def embed(m, cast=False):
+        out = []
+        with torch.inference_mode():
+            for b in batches:
+                b = {k: v.float() if cast and v.is_floating_point() else v for k, v in b.items()}
+                out.append(m(**b).embeddings.float().clone())
+        return out
+
+    exact, before = embed(wide, True), embed(model)
+    calls = {"attention": 0, "turned": 0}
+    attention, launch = ea.attention, ea._launch_rotary
+    monkeypatch.setattr(ea, "attention", lambda *a, **k: (calls.__setitem__("attention", calls["attention"] + 1), attention(*a, **k))[1])
+    monkeypatch.setattr(ea, "_launch_rotary", lambda *a, **k: (calls.__setitem__("turned", calls["turned"] + 1), launch(*a, **k))[1])
+    counts = ea.patch_attention(model)
+    got = embed(model)
+    layers = len([m for m in model.modules() if type(m).__name__ in ("GemmaAttention", "Qwen2VLAttention", "Qwen2_5_VLAttention")])
+    vision = len([m for m in model.modules() if type(m).__name__ in ("SiglipAttention", "VisionAttention", "Qwen2_5_VLVisionAttention")])
+    assert counts["rotary"] == 1 and counts["decoder"] == layers and counts["packed"] == (0 if kind == "colpali" else vision)
+    assert calls["attention"] == 3 * layers + vision and calls["turned"] == 3 * layers + counts["packed"]
+    for b, x, y, z in zip(batches, exact, before, got):
+        valid = b["attention_mask"].bool()
+        off, base = (z - x)[valid].norm(dim=-1), (y - x)[valid].norm(dim=-1)
+        print(f"{kind}: off the float32 model by {float(off.max()):.4f} (unpatched {float(base.max()):.4f})")
+        assert float(off.max()) <= 1.5 * float(base.max()) + 4 * 2.0**-8 and bool(torch.isfinite(z).all())
+    with torch.enable_grad():  # autograd on: the modules' own forwards
+        n = dict(calls)
+        assert model(**batches[0]).embeddings.requires_grad and calls == n
+    ea.unpatch_attention(model)
+    assert all(torch.equal(a, b) for a, b in zip(embed(model), before))
+
+
+def test_embedding_model_with_fused_attention(ea):
+    """The option of the embedding class, end to end: pages and queries, as many rows as without it and nearly the same directions."""
+    import asyncio
+
+    from morphik_core_amd.embedding import MI355XColpaliEmbeddingModel
+
+    plain = MI355XColpaliEmbeddingModel(preset="tiny", device="cuda", seed=1)
+    fused = MI355XColpaliEmbeddingModel(preset="tiny", device="cuda", seed=1, fused_attention=True)
+    assert plain.fused_attention == {"rotary": 0, "decoder": 0, "packed": 0} and fused.fused_attention == {"rotary": 1, "decoder": 2, "packed": 0}
+    for text in ("revenue", "what is the total revenue of the second quarter"):
+        a, b = (asyncio.run(m.embed_for_query(text)) for m in (plain, fused))
+        assert a.shape == b.shape and float((a * b).sum(-1).min()) > 0.99

@@ -44,6 +44,7 @@ constexpr int block_waves(int kc) { return kc == 5 || kc == 6 ? 4 : 8; }
 constexpr int block_rows(int kc) { return block_waves(kc) * kWaveRows; }
 // The widths that are built: a head takes the next wider one
 constexpr int built_kc(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : dim <= 128 ? 8 : dim <= 192 ? 12 : 16; }
+constexpr int kMatrix = 0x008, kDsRead = 0x100;  // classes of __builtin_amdgcn_sched_group_barrier
 constexpr float kRescale = 8.f;                // running maxima move only when a score passes them by 2^8: the weights stay <= 256
 
 constexpr int64_t kMaxRowStride = 1 << 23;    // elements: a tile's byte offsets stay below 2^31
@@ -127,7 +128,8 @@ __device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* 
 }
 
 // Where a 16-byte chunk of a staged row lies: chunk c of row r at r * CH + (c ^ swizzle(r)).  LDS serves 256 bytes a cycle: 16 lanes of a K read
-// (one row each, the same column) and 32 lanes of a V read (four rows x four chunks each) have to meet all 16 chunk positions.
+// (one row each, the same column) and 32 lanes of a V read (four rows x four chunks each) have to meet all 16 chunk positions.  Measured: no
+// conflict at any width.
 template <int CH>
 __device__ __forceinline__ int swizzle_k(int r) {
   if constexpr (CH % 16 == 0) return r & 15;
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
   constexpr int VC = DT * 4;                   // and of a staged row of V (the last tile's unused columns hold anything: their results are dropped)
   constexpr int kThreads = kWaves * 64;
   constexpr int kLoadsK = (BK * CH + kThreads - 1) / kThreads, kLoadsV = (BK * VC + kThreads - 1) / kThreads;
-  __shared__ __attribute__((aligned(1024))) u32x4 lds_k[2][BK * CH], lds_v[2][BK * VC];
+  __shared__ u32x4 lds_k[2][BK * CH], lds_v[2][BK * VC];
   __shared__ int lds_range[kWaves][2];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
 
@@ -199,9 +201,12 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
   const uint16_t* vb = a.v + b * a.v_b + hk * a.v_h;
 
   // this lane's row
-  const int64_t r = (int64_t)tile * kBlockRows + wave * kWaveRows + (lane & 31);
-  const bool live = r < (int64_t)a.rows * a.group;
-  const int pos = live ? (int)(r / a.group) : 0, head = hk * a.group + (live ? (int)(r % a.group) : 0);
+  const uint32_t all = (uint32_t)a.rows * (uint32_t)a.group;  // below 2^31
+  // keys that some row of the wave sees [w_lo, w_hi), that every row sees [in_lo, in_hi); the block's tiles cover all waves'
+  int w_lo = 0x7fffffff, w_hi = 0, in_lo = 0, in_hi = 0x7fffffff;
+  const uint32_t r = (uint32_t)tile * kBlockRows + wave * kWaveRows + (lane & 31);
+  const bool live = r < all;
+  const int pos = live ? (int)(r / (uint32_t)a.group) : 0, head = hk * a.group + (live ? (int)(r % (uint32_t)a.group) : 0);
   int lo = 0, hi = live ? a.keys : 0;
   if (live && a.ranges) {
     const int2 rg = *reinterpret_cast<const int2*>(a.ranges + b * a.range_b + (int64_t)pos * 2);
@@ -210,11 +215,12 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
   } else if (live && a.causal) {
     hi = (int)min((int64_t)pos + 1 + a.keys - a.rows, (int64_t)a.keys);
   }
-  if (lo >= hi) lo = hi = 0;
-  const bool empty = lo == hi;
-
-  // keys that some row of the wave sees [w_lo, w_hi), that every row sees [in_lo, in_hi); the block's tiles cover all waves'
-  int w_lo = empty ? 0x7fffffff : lo, w_hi = hi, in_lo = lo, in_hi = empty ? 0x7fffffff : hi;
+  if (lo >= hi) {
+    lo = hi = 0;
+  } else {
+    w_lo = in_lo = lo;
+    w_hi = in_hi = hi;
+  }
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
     w_lo = min(w_lo, __shfl_xor(w_lo, s));
@@ -235,12 +241,18 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     k_hi = max(k_hi, lds_range[w][1]);
   }
   k_lo = uniform(k_lo), k_hi = uniform(k_hi);
-  int lo_s = lo, hi_s = hi;  // what this block sees of the row's range
   if (partial) {
-    const int share = ((k_hi - k_lo + BK - 1) / BK + a.splits - 1) / a.splits * BK;  // whole tiles
-    k_lo = k_lo < k_hi ? (int)min((int64_t)k_lo + (int64_t)split * share, (int64_t)k_hi) : 0;
-    k_hi = min((int64_t)k_lo + share, (int64_t)k_hi);
-    lo_s = max(lo, k_lo), hi_s = min(hi, k_hi);
+    const int tiles = (k_hi - k_lo + BK - 1) / BK;
+    const int pieces = max(min(a.splits, tiles / 2), 1);  // short ranges stay in one piece, and are told apart by a sum of -1
+    if (pieces == 1) {
+      if (split) return;
+      if (live && half == 0) *reinterpret_cast<float2*>(partial + (wave * kWaveRows + lane) * (a.dim + 4) + a.dim) = make_float2(-INFINITY, -1.f);
+      partial = nullptr;
+    } else {
+      const int share = (tiles + pieces - 1) / pieces * BK;  // whole tiles
+      k_lo = (int)min((int64_t)k_lo + (int64_t)split * share, (int64_t)k_hi);
+      k_hi = (int)min((int64_t)k_lo + share, (int64_t)k_hi);
+    }
   }
 
   // q: the columns 16 kk + 8 half ... + 7 of this lane's row
@@ -250,6 +262,12 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
   for (int kk = 0; kk < KC; ++kk) {
     const int c = kk * 16 + half * 8;
     qf[kk] = live && c < a.dim ? *reinterpret_cast<const s16x8*>(qr + c) : s16x8{};
+  }
+  // Arrived before the tiles' loads start: the compiler would wait for q inside the loop, and with it for the tile just sent for (8464 rows of heads of
+  // 80: 479 -> 447 us).  Heads of 256 have no registers to spare for that and are faster without (160 and 150 us).
+  if constexpr (KC <= 12) {
+#pragma unroll
+    for (int kk = 0; kk < KC; ++kk) asm volatile("" : "+v"(qf[kk]));
   }
 
   // staging: thread t moves the chunks at positions t, t + kThreads, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
@@ -287,6 +305,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
 
   f32x16 o[DT] = {};
   float m = -INFINITY, l = 0.f;
+  const float qk = CAP ? 1.f : a.qk;  // capped scores are logarithms already
   if (k_lo < k_hi) fetch(k_lo, 0);
 
   int buf = 0;
@@ -302,17 +321,29 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     for (int t = 0; t < BK / 32; ++t) {
       const int row = t * 32 + (lane & 31);
 #pragma unroll
-      for (int kk = 0; kk < KC; ++kk)
-        s[t] = mfma<BF16>(*reinterpret_cast<const s16x8*>(lk + (row * CH + ((kk * 2 + half) ^ swizzle_k<CH>(row))) * 8), qf[kk], s[t]);
+      for (int kk = 0; kk < KC; ++kk) {
+        const s16x8 kf = *reinterpret_cast<const s16x8*>(lk + (row * CH + ((kk * 2 + half) ^ swizzle_k<CH>(row))) * 8);
+        s[t] = mfma<BF16>(kf, qf[kk], s[t]);
+      }
+    }
+    if constexpr (KC <= 12) {  // reads run ahead of their products (left to itself the compiler waits for each; heads of 128: 261 -> 252 us)
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 1);
+#pragma unroll
+      for (int n = 0; n < KC * BK / 32; ++n) {
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
+      }
     }
 
+    const bool cut = k0 < in_lo || k0 + BK > in_hi;  // some row does not see some key of the tile
+    s16x8 p[BK / 16];
     if constexpr (CAP) {
 #pragma unroll
       for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] = score<true>(s[t][e], a.qk, a.cap);
     }
-    if (k0 < in_lo || k0 + BK > in_hi) {  // some row does not see some key of the tile
+    if (cut) {
 #pragma unroll
       for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
@@ -326,9 +357,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float qk = CAP ? 1.f : a.qk;  // capped scores are logarithms already
-    top *= qk;
+    top = fmaxf(top, __shfl_xor(top, 32)) * qk;
     if (__any(top > m + kRescale)) {
       const float m2 = fmaxf(m, top);
       const float alpha = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
@@ -341,7 +370,6 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     }
     const float base = m == -INFINITY ? 0.f : m;
     // weights, rounded to the operands' type for the matrix instruction (half a step of it, below the output's own rounding)
-    s16x8 p[BK / 16];
 #pragma unroll
     for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
@@ -365,40 +393,54 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
         uint16_t* src = lv + (row * VC + (chunk ^ swizzle_v<VC>(row))) * 8 + 4 * (lane & 1);
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
         const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 8 * VC * 8));
-        o[d] = mfma<BF16>(__builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7), p[c], o[d]);
+        const s16x8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = mfma<BF16>(vf, p[c], o[d]);
       }
+    if constexpr (KC <= 12) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 0);
+#pragma unroll
+      for (int n = 0; n < DT * BK / 16; ++n) {
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+      }
+    }
   }
 
   l += __shfl_xor(l, 32);
-  uint16_t* orow = a.out + b * a.o_b + (int64_t)pos * a.o_l + head * a.o_h;
-  float* prow = partial + (wave * kWaveRows + (lane & 31)) * (a.dim + 4);
+  const int lo_s = max(lo, k_lo), hi_s = min(hi, k_hi);  // what this block saw of the row's range
   const bool nothing = lo_s >= hi_s;
   const float inv = partial ? 1.f : 1.f / l;
-  bool bad = false;
+  float odd = 0.f;  // NaN from the first value on that is not finite
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      o[d][e] = nothing ? 0.f : o[d][e] * inv;
-      if (d * 32 + e / 4 * 8 < a.dim) bad |= !(fabsf(o[d][e]) < INFINITY);
+      o[d][e] *= inv;
+      if (d * 32 + e / 4 * 8 < a.dim) odd = __builtin_fmaf(o[d][e], 0.f, odd);
     }
-  bad &= live;
+  const bool bad = live && !nothing && odd != odd;
+  uint16_t* orow = a.out + b * a.o_b + (int64_t)pos * a.o_l + head * a.o_h;
+  float* prow = partial + (wave * kWaveRows + (lane & 31)) * (a.dim + 4);
   // columns 32 d + 8 e + 4 half + 0..3 of this lane's row
   if (!partial) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (d * 32 + e * 8 < a.dim && live)
-          *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = u32x2{pack2<BF16>(o[d][e * 4], o[d][e * 4 + 1]), pack2<BF16>(o[d][e * 4 + 2], o[d][e * 4 + 3])};
-  } else {
-    if (live && half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
+        if (d * 32 + e * 8 < a.dim && live) {
+          const u32x2 w = {pack2<BF16>(o[d][e * 4], o[d][e * 4 + 1]), pack2<BF16>(o[d][e * 4 + 2], o[d][e * 4 + 3])};
+          *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = nothing ? u32x2{0, 0} : w;
+        }
+  } else if (live) {
+    if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
+    if (!nothing) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (d * 32 + e * 8 < a.dim && live && !nothing)
-          *reinterpret_cast<f32x4*>(prow + d * 32 + e * 8 + half * 4) = f32x4{o[d][e * 4], o[d][e * 4 + 1], o[d][e * 4 + 2], o[d][e * 4 + 3]};
+        for (int e = 0; e < 4; ++e)
+          if (d * 32 + e * 8 < a.dim)
+            *reinterpret_cast<f32x4*>(prow + d * 32 + e * 8 + half * 4) = f32x4{o[d][e * 4], o[d][e * 4 + 1], o[d][e * 4 + 2], o[d][e * 4 + 3]};
+    }
   }
   uint64_t again = __ballot(bad);
   again = (again | again >> 32) & 0xffffffffu;
@@ -429,6 +471,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
   const bool live = in_tile < stored && r < all;  // of the whole group of W waves
   const int64_t step = (int64_t)stored * (a.dim + 4);
   const float* src = a.partial + (int64_t)cut * a.splits * step + (int64_t)(live ? in_tile : 0) * (a.dim + 4);
+  if (src[a.dim + 1] == -1.f) return;  // not in pieces after all: the row is done (W waves see the same row, and end together)
   float m = -INFINITY, l = 0.f;
   f32x4 o = {};
   if (live) {
@@ -446,9 +489,9 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
 #pragma unroll 8
       for (int i = wave % W; i < n; i += W) {
         const float wi = __shfl(w, i);
-        const f32x4 part = lane * 4 < a.dim ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
+        const f32x4 part = lane * 4 < a.dim && wi != 0.f ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = wi == 0.f ? o[e] : __builtin_fmaf(part[e], wi, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(part[e], wi, o[e]);
       }
     }
 #pragma unroll
@@ -471,7 +514,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
 
 template <bool BF16>
 void launch_join(const AttnArgs& a, int64_t cut, int64_t stored, hipStream_t s) {
-  if (a.splits >= 16) hipLaunchKernelGGL((join_kernel<BF16, 4>), dim3((unsigned)(cut * stored)), dim3(256), 0, s, a);
+  if (a.splits >= 16 && cut * stored <= 2048) hipLaunchKernelGGL((join_kernel<BF16, 4>), dim3((unsigned)(cut * stored)), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((join_kernel<BF16, 1>), dim3((unsigned)(cut * ((stored + 3) / 4))), dim3(256), 0, s, a);
 }
 
@@ -635,7 +678,7 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   const int64_t tall = (int64_t)p->rows * a.group;  // rows of one K/V head
   const Plan pl = plan(p->batch, p->rows, p->keys, p->heads, p->kv_heads, p->dim, cu_count(device));
   const int64_t blocks = pl.full + pl.cut * pl.splits;
-  if (pl.blocks > 0x7fffffff || blocks > 0x7fffffff) {
+  if (tall > 0x7ffff000 || pl.blocks > 0x7fffffff || blocks > 0x7fffffff) {
     set_error("mv_enc_attention: too many rows for one launch");
     return MV_ERR_INVALID;
   }

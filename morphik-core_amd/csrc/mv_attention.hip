@@ -34,7 +34,8 @@ using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaveRows = 32;                  // rows of a wave: the N of the 32x32x16 matrix instruction
 constexpr int kXcds = 8;
-// By KC, the 16-column steps of a head.  Keys of a tile: two products deep where the registers allow it.  Waves of a SIMD at once: by registers.
+// By KC, the 16-column steps of a head.  Keys of a tile: two products deep where the registers allow it.  Waves of a SIMD at once: by registers; heads of
+// 72 ... 96 would fit three, which is slower (8464 rows of heads of 80: 444 us with two, 475 with three).
 // Waves of a block: eight share a tile's loads (2 x 4096 rows, heads of 128: 278 us with four, 270 with eight; 4 x 2048 of 256: 163 and 146), but for
 // heads of 72 ... 96, whose tiles do not divide evenly among 512 threads and which vision towers use with short windows (heads of 80: 8464 rows 467 us
 // with four, 543 with eight; windows of 64 rows 64 and 78).
@@ -169,7 +170,8 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // Tiles are double-buffered: while one is computed the next is on its way from memory to LDS, and one barrier a tile both publishes the
 // arrived one and frees the other.
 template <bool BF16, int KC, bool CAP>
-__global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(KC), waves_per_simd(KC)))) void attention_kernel(
+    const AttnArgs a) {
   constexpr int kWaves = block_waves(KC), kBlockRows = block_rows(KC);
   constexpr int BK = tile_keys(KC);
   constexpr int DT = (KC + 1) / 2;             // 32-column tiles of the output; KC: 16-column steps of q.k
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
   int w_lo = 0x7fffffff, w_hi = 0, in_lo = 0, in_hi = 0x7fffffff;
   const uint32_t r = (uint32_t)tile * kBlockRows + wave * kWaveRows + (lane & 31);
   const bool live = r < all;
-  const int pos = live ? (int)(r / (uint32_t)a.group) : 0, head = hk * a.group + (live ? (int)(r % (uint32_t)a.group) : 0);
+  int pos = live ? (int)(r / (uint32_t)a.group) : 0, head = hk * a.group + (live ? (int)(r % (uint32_t)a.group) : 0);
   int lo = 0, hi = live ? a.keys : 0;
   if (live && a.ranges) {
     const int2 rg = *reinterpret_cast<const int2*>(a.ranges + b * a.range_b + (int64_t)pos * 2);
@@ -270,37 +272,47 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     for (int kk = 0; kk < KC; ++kk) asm volatile("" : "+v"(qf[kk]));
   }
 
-  // staging: thread t moves the chunks at positions t, t + kThreads, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
-  // one copies of the first (a row that is finite stays so; the weights and the columns of q there are zero)
+  // Staging: thread t moves the chunks at positions t, t + kThreads, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
+  // one copies of the first (a row that is finite stays so; the weights and the columns of q there are zero).  Where kThreads positions are whole rows and
+  // whole periods of the swizzle, the chunks of a thread differ by whole rows: one register of offsets, but for the last tile.
+  constexpr bool kEven = kThreads % CH == 0 && kThreads / CH % 16 == 0 && VC == CH;
+  constexpr int kOffsets = kEven ? 1 : (kLoadsK > kLoadsV ? kLoadsK : kLoadsV);
   const uint32_t k_step = (uint32_t)a.k_l * 2, v_step = (uint32_t)a.v_l * 2;
-  auto place = [&](int i, int n, int sw, uint32_t step, int last) {
-    const int row = i / n;
-    int c = i % n ^ sw;
-    c = c * 8 < a.dim ? c : 0;
-    return (uint32_t)min(row, last) * step + (uint32_t)c * 16;
+  auto place_k = [&](int n, int last) {
+    const int i = n * kThreads + threadIdx.x, row = i / CH, c = i % CH ^ swizzle_k<CH>(row);
+    return (uint32_t)min(row, last) * k_step + (c * 8 < a.dim ? c * 16 : 0);
   };
-  uint32_t k_off[kLoadsK], v_off[kLoadsV];
-  auto offsets = [&](int last) {
-#pragma unroll
-    for (int n = 0; n < kLoadsK; ++n) k_off[n] = place(n * kThreads + threadIdx.x, CH, swizzle_k<CH>((n * kThreads + threadIdx.x) / CH), k_step, last);
-#pragma unroll
-    for (int n = 0; n < kLoadsV; ++n) v_off[n] = place(n * kThreads + threadIdx.x, VC, swizzle_v<VC>((n * kThreads + threadIdx.x) / VC), v_step, last);
+  auto place_v = [&](int n, int last) {
+    const int i = n * kThreads + threadIdx.x, row = i / VC, c = i % VC ^ swizzle_v<VC>(row);
+    return (uint32_t)min(row, last) * v_step + (c * 8 < a.dim ? c * 16 : 0);
   };
-  offsets(BK);
+  uint32_t k_off[kOffsets], v_off[kOffsets];
+#pragma unroll
+  for (int n = 0; n < kOffsets; ++n) k_off[n] = place_k(n, BK), v_off[n] = place_v(n, BK);
   const uint16_t *kt = kb + (int64_t)k_lo * a.k_l, *vt = vb + (int64_t)k_lo * a.v_l;  // of the tile sent for next
-  const int64_t kt_step = a.k_l * BK, vt_step = a.v_l * BK;
   const uint32_t dk = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_k[0][wave * 64]), dv = uniform((uint32_t)(uintptr_t)(lds_u32x4*)&lds_v[0][wave * 64]);
   auto fetch = [&](int k0, int buf) {
-    if (k0 + BK > k_hi) offsets(k_hi - 1 - k0);
     const uint32_t sk = dk + buf * (BK * CH * 16), sv = dv + buf * (BK * VC * 16);
+    const int last = k_hi - 1 - k0;
+    if (last >= BK - 1) {
 #pragma unroll
-    for (int n = 0; n < kLoadsK; ++n)
-      if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH) dma16(kt, k_off[n], sk + n * kThreads * 16);
+      for (int n = 0; n < kLoadsK; ++n)
+        if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH)
+          dma16(kEven ? kt + n * (kThreads / CH) * a.k_l : kt, k_off[kEven ? 0 : n], sk + n * kThreads * 16);
 #pragma unroll
-    for (int n = 0; n < kLoadsV; ++n)
-      if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC) dma16(vt, v_off[n], sv + n * kThreads * 16);
-    kt += kt_step;
-    vt += vt_step;
+      for (int n = 0; n < kLoadsV; ++n)
+        if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC)
+          dma16(kEven ? vt + n * (kThreads / VC) * a.v_l : vt, v_off[kEven ? 0 : n], sv + n * kThreads * 16);
+    } else {
+#pragma unroll
+      for (int n = 0; n < kLoadsK; ++n)
+        if ((n + 1) * kThreads <= BK * CH || n * kThreads + wave * 64 < BK * CH) dma16(kt, place_k(n, last), sk + n * kThreads * 16);
+#pragma unroll
+      for (int n = 0; n < kLoadsV; ++n)
+        if ((n + 1) * kThreads <= BK * VC || n * kThreads + wave * 64 < BK * VC) dma16(vt, place_v(n, last), sv + n * kThreads * 16);
+    }
+    kt += a.k_l * BK;
+    vt += a.v_l * BK;
   };
 
   f32x16 o[DT] = {};
@@ -326,13 +338,12 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
         s[t] = mfma<BF16>(kf, qf[kk], s[t]);
       }
     }
-    if constexpr (KC <= 12) {  // reads run ahead of their products (left to itself the compiler waits for each; heads of 128: 261 -> 252 us)
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 1);
+    // reads run ahead of their products, as far as there are registers (left to itself the compiler waits for each; heads of 128: 261 -> 252 us)
+    __builtin_amdgcn_sched_group_barrier(kDsRead, KC > 12 ? 3 : 6, 1);
 #pragma unroll
-      for (int n = 0; n < KC * BK / 32; ++n) {
-        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
-      }
+    for (int n = 0; n < KC * BK / 32; ++n) {
+      __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
     }
 
     const bool cut = k0 < in_lo || k0 + BK > in_hi;  // some row does not see some key of the tile
@@ -396,17 +407,19 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
         const s16x8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         o[d] = mfma<BF16>(vf, p[c], o[d]);
       }
-    if constexpr (KC <= 12) {
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, KC > 12 ? 4 : 8, 0);
 #pragma unroll
-      for (int n = 0; n < DT * BK / 16; ++n) {
-        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
-      }
+    for (int n = 0; n < DT * BK / 16; ++n) {
+      __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
     }
   }
 
   l += __shfl_xor(l, 32);
+  uint32_t again_r = (uint32_t)tile * kBlockRows + threadIdx.x / 64 * kWaveRows + (threadIdx.x & 31);
+  asm("" : "+v"(again_r));  // the row once more: two registers less across the loop
+  const bool live_e = again_r < all;
+  pos = live_e ? (int)(again_r / (uint32_t)a.group) : 0, head = hk * a.group + (live_e ? (int)(again_r % (uint32_t)a.group) : 0);
   const int lo_s = max(lo, k_lo), hi_s = min(hi, k_hi);  // what this block saw of the row's range
   const bool nothing = lo_s >= hi_s;
   const float inv = partial ? 1.f : 1.f / l;
@@ -418,7 +431,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
       o[d][e] *= inv;
       if (d * 32 + e / 4 * 8 < a.dim) odd = __builtin_fmaf(o[d][e], 0.f, odd);
     }
-  const bool bad = live && !nothing && odd != odd;
+  const bool bad = live_e && !nothing && odd != odd;
   uint16_t* orow = a.out + b * a.o_b + (int64_t)pos * a.o_l + head * a.o_h;
   float* prow = partial + (wave * kWaveRows + (lane & 31)) * (a.dim + 4);
   // columns 32 d + 8 e + 4 half + 0..3 of this lane's row
@@ -427,11 +440,11 @@ __global__ __launch_bounds__(block_waves(KC) * 64, waves_per_simd(KC)) void atte
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (d * 32 + e * 8 < a.dim && live) {
+        if (d * 32 + e * 8 < a.dim && live_e) {
           const u32x2 w = {pack2<BF16>(o[d][e * 4], o[d][e * 4 + 1]), pack2<BF16>(o[d][e * 4 + 2], o[d][e * 4 + 3])};
           *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = nothing ? u32x2{0, 0} : w;
         }
-  } else if (live) {
+  } else if (live_e) {
     if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
     if (!nothing) {
 #pragma unroll

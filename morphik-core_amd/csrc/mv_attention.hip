@@ -209,6 +209,14 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
   const uint32_t r = (uint32_t)tile * kBlockRows + wave * kWaveRows + (lane & 31);
   const bool live = r < all;
   int pos = live ? (int)(r / (uint32_t)a.group) : 0, head = hk * a.group + (live ? (int)(r % (uint32_t)a.group) : 0);
+  // q: the columns 16 kk + 8 half ... + 7 of this lane's row
+  const uint16_t* qr = a.q + b * a.q_b + (int64_t)pos * a.q_l + head * a.q_h;
+  s16x8 qf[KC];
+#pragma unroll
+  for (int kk = 0; kk < KC; ++kk) {
+    const int c = kk * 16 + half * 8;
+    qf[kk] = live && c < a.dim ? *reinterpret_cast<const s16x8*>(qr + c) : s16x8{};
+  }
   int lo = 0, hi = live ? a.keys : 0;
   if (live && a.ranges) {
     const int2 rg = *reinterpret_cast<const int2*>(a.ranges + b * a.range_b + (int64_t)pos * 2);
@@ -257,14 +265,6 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
     }
   }
 
-  // q: the columns 16 kk + 8 half ... + 7 of this lane's row
-  const uint16_t* qr = a.q + b * a.q_b + (int64_t)pos * a.q_l + head * a.q_h;
-  s16x8 qf[KC];
-#pragma unroll
-  for (int kk = 0; kk < KC; ++kk) {
-    const int c = kk * 16 + half * 8;
-    qf[kk] = live && c < a.dim ? *reinterpret_cast<const s16x8*>(qr + c) : s16x8{};
-  }
   // Arrived before the tiles' loads start: the compiler would wait for q inside the loop, and with it for the tile just sent for (8464 rows of heads of
   // 80: 479 -> 447 us).  Heads of 256 have no registers to spare for that and are faster without (160 and 150 us).
   if constexpr (KC <= 12) {

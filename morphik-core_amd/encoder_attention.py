@@ -461,7 +461,8 @@ def _interface_attention(module, query, key, value, attention_mask=None, scaling
     causal = getattr(module, "is_causal", False) if is_causal is None else is_causal
     causal = bool(causal) and attention_mask is None and query.shape[2] > 1
     known = ranges is not None or attention_mask is None and not (causal and query.shape[2] != key.shape[2])
-    if known and not dropout and _kernel_takes(torch, query, key, value):
+    extras = any(kwargs.get(name) is not None for name in ("s_aux", "position_bias"))  # sinks, added biases: not in the kernel
+    if known and not dropout and not extras and _kernel_takes(torch, query, key, value):
         out = attention(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), key_ranges=ranges, causal=causal, scale=scaling, softcap=softcap or 0.0)
         return out, None
     from transformers import AttentionInterface

@@ -181,6 +181,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
   constexpr int kLoadsK = (BK * CH + kThreads - 1) / kThreads, kLoadsV = (BK * VC + kThreads - 1) / kThreads;
   __shared__ u32x4 lds_k[2][BK * CH], lds_v[2][BK * VC];
   __shared__ int lds_range[kWaves][2];
+  __shared__ int2 lds_rows[kBlockRows];  // the rows' key ranges: two registers less in the loop, where heads of 256 have none to spare (144 -> 136 us)
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
 
   // Blocks of one K/V head next to each other on one XCD (its L2 then holds that head's keys once): consecutive block numbers go round the XCDs, so
@@ -243,6 +244,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
     lds_range[wave][0] = w_lo;
     lds_range[wave][1] = w_hi;
   }
+  if (half == 0) lds_rows[wave * kWaveRows + lane] = make_int2(lo, hi);
   __syncthreads();
   int k_lo = 0x7fffffff, k_hi = 0;
 #pragma unroll
@@ -251,6 +253,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
     k_hi = max(k_hi, lds_range[w][1]);
   }
   k_lo = uniform(k_lo), k_hi = uniform(k_hi);
+  if (k_lo >= k_hi) k_lo = k_hi = 0;  // no row of the block sees anything: positions stay far from the end of 32 bits
   if (partial) {
     const int tiles = (k_hi - k_lo + BK - 1) / BK;
     const int pieces = max(min(a.splits, tiles / 2), 1);  // short ranges stay in one piece, and are told apart by a sum of -1
@@ -355,12 +358,13 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
         for (int e = 0; e < 16; ++e) s[t][e] = score<true>(s[t][e], a.qk, a.cap);
     }
     if (cut) {
+      const int2 row = lds_rows[wave * kWaveRows + (lane & 31)];
 #pragma unroll
       for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int key = k0 + t * 32 + 8 * (e / 4) + 4 * half + e % 4;
-          s[t][e] = key >= lo && key < hi ? s[t][e] : -INFINITY;
+          s[t][e] = key >= row.x && key < row.y ? s[t][e] : -INFINITY;
         }
     }
     float top = s[0][0];
@@ -420,7 +424,8 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
   asm("" : "+v"(again_r));  // the row once more: two registers less across the loop
   const bool live_e = again_r < all;
   pos = live_e ? (int)(again_r / (uint32_t)a.group) : 0, head = hk * a.group + (live_e ? (int)(again_r % (uint32_t)a.group) : 0);
-  const int lo_s = max(lo, k_lo), hi_s = min(hi, k_hi);  // what this block saw of the row's range
+  const int2 row = lds_rows[wave * kWaveRows + (lane & 31)];
+  const int lo_s = max(row.x, k_lo), hi_s = min(row.y, k_hi);  // what this block saw of the row's range
   const bool nothing = lo_s >= hi_s;
   const float inv = partial ? 1.f : 1.f / l;
   float odd = 0.f;  // NaN from the first value on that is not finite
@@ -637,7 +642,7 @@ using namespace mv;
 extern "C" {
 
 int mv_enc_attention(int device, const mv_attn* p, void* stream) {
-  if (!p || p->batch < 0 || p->rows < 0 || p->keys < 0 || p->keys > 0x7fffff00 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads) {
+  if (!p || p->batch < 0 || p->rows < 0 || p->keys < 0 || p->keys > 0x7ffff000 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads) {
     set_error("mv_enc_attention: bad sizes (heads must be a positive multiple of kv_heads)");
     return MV_ERR_INVALID;
   }

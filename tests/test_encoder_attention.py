@@ -199,7 +199,7 @@ def test_the_c_entries_refuse_bad_structs_before_any_launch():
         return L.mv_enc_attention(0, C.byref(p), None), L.mv_last_error().decode()
 
     assert attn(batch=0)[0] == 0 and attn(rows=0)[0] == 0  # nothing to do is no error
-    for kw in (dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(batch=-1), dict(keys=-1), dict(keys=0x7FFFFFFF), dict(dtype=_lib.MV_F32), dict(dim=20),
+    for kw in (dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(batch=-1), dict(keys=-1), dict(keys=0x7FFFF001), dict(dtype=_lib.MV_F32), dict(dim=20),
                dict(dim=0), dict(dim=264), dict(scale=0.0), dict(scale=math.inf), dict(softcap=-1.0), dict(q=0), dict(k=8), dict(out=20),
                dict(q_row=4), dict(v_head=12), dict(ranges=4), dict(ranges=8, ranges_batch=3), dict(rows=0x7FFFFFFF, heads=4096, kv_heads=1)):
         rc, msg = attn(**kw)

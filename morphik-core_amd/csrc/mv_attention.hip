@@ -268,12 +268,10 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
     }
   }
 
-  // Arrived before the tiles' loads start: the compiler would wait for q inside the loop, and with it for the tile just sent for (8464 rows of heads of
-  // 80: 479 -> 447 us).  Heads of 256 have no registers to spare for that and are faster without (160 and 150 us).
-  if constexpr (KC <= 12) {
+  // q has arrived before the tiles' loads start: the compiler would wait for it inside the loop, and with it for the tile just sent for (8464 rows of heads
+  // of 80: 479 -> 447 us)
 #pragma unroll
-    for (int kk = 0; kk < KC; ++kk) asm volatile("" : "+v"(qf[kk]));
-  }
+  for (int kk = 0; kk < KC; ++kk) asm volatile("" : "+v"(qf[kk]));
 
   // Staging: thread t moves the chunks at positions t, t + kThreads, ... of a tile.  Rows behind the last key are copies of it, columns behind the last
   // one copies of the first (a row that is finite stays so; the weights and the columns of q there are zero).  Where kThreads positions are whole rows and

@@ -11,6 +11,7 @@ Only what the hot path needs:
   store_server.py  one HBM slab, many processes: owner server + MI355XRemoteMultiVectorStore
   embedding.py   MI355XColpaliEmbeddingModel: BaseEmbeddingModel plugin (PyTorch-ROCm encoder, device-resident ingest)
   colqwen_embedding.py  MI355XColQwen2EmbeddingModel: the reference's encoder family (dynamic patch counts -> ragged pages)
+  encoder_ops.py / encoder_attention.py  the encoders' block operators as HIP kernels: norms and activations; rotary positions and attention
   embed_server.py  the reference's /embeddings npz protocol served from an MI355X (one server per GPU)
   formats.py     importers for the reference's formats: .npy page tree, .npz wire format, BIT(128)[] rows
   sharded.py     row-sharded corpus over N ranks (one process per GPU), RCCL all-gather of per-shard top-k

@@ -168,7 +168,14 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // transposing read: 16 lanes that address four keys x 16 columns get one column each, four keys deep.
 //
 // Tiles are double-buffered: while one is computed the next is on its way from memory to LDS, and one barrier a tile both publishes the
-// arrived one and frees the other.
+// arrived one and frees the other (three or four places instead of two: no gain at any width).
+//
+// What bounds it: a SIMD's two waves share the matrix unit and the vector unit, and neither is busy more than half of the time -- reads of LDS, the
+// exchange of maxima and the barrier leave gaps that two waves do not fill; three do not fit the registers.  One MI355X, whose library reaches 1.30
+// PFLOP/s in a large bf16 product: 2 x 4096 rows of 16 heads of 128 254 us (1.08 PFLOP/s), of 64 150 us (0.92), 4 x 2048 rows of 8 heads of 256 over one
+// K/V head 133 us (1.03), 8464 rows of 16 heads of 80 444 us (0.83; the 16-column and 32-column steps round 80 up to 80 and 96).  Tried and not kept: two
+// groups of waves half a tile apart (289 us at 128), the weights of 32 keys beside the products of the next 32 (292), 64 rows a wave
+// (289, and 209 at 256), wave priorities (no change).
 template <bool BF16, int KC, bool CAP>
 __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(KC), waves_per_simd(KC)))) void attention_kernel(
     const AttnArgs a) {

@@ -35,19 +35,11 @@ struct RotaryArgs {
   float scale;
   int32_t batch, rows, heads, kv_heads, dim, pairs, tokens;  // tokens: of a block
   int64_t total;                             // batch * rows
-  int32_t pos64, copy_rest;                  // copy_rest: elements from 2 * pairs on are written too (not when in place)
+  int32_t pos64;
+  int32_t rot_vecs, rot_ones, copy_vecs, copy_ones;  // work items of a head: vectors and single pairs that turn, vectors and elements that are copied
 };
 
-template <int N>
-struct Bytes;
-template <>
-struct Bytes<2> { using type = uint16_t; };
-template <>
-struct Bytes<4> { using type = uint32_t; };
-template <>
-struct Bytes<16> { using type = __attribute__((ext_vector_type(4))) unsigned int; };
-
-// T: 0 fp32, 1 bf16, 2 fp16.  VE elements at a time: 16 bytes, or one where the sizes or alignments do not allow that.
+// T: 0 fp32, 1 bf16, 2 fp16
 template <int T>
 struct Elem;
 template <>
@@ -57,16 +49,35 @@ struct Elem<1> { using type = __bf16; };
 template <>
 struct Elem<2> { using type = _Float16; };
 
-template <int T, int VE, bool ADJ>
+// Items of 16 bytes whatever the alignment: heads of 72 have 36 pairs, so that the second halves start in the middle of 16 bytes, and odd numbers of pairs
+// in the middle of a word.  Such loads and stores are single instructions too (element alignment is what they are compiled for).  Against items of one
+// element wherever 16 bytes are not aligned, bf16: 12512 tokens x 32 heads of 72 57.8 -> 20.9 us, 8 x 1101 x 18 heads of 128 with 33 pairs 60.8 -> 18.5
+// (adjacent 73.3 -> 19.1, in place 28.9 -> 16.8).
+template <class E>
+__device__ __forceinline__ void load(E (&v)[16 / sizeof(E)], const E* p) { __builtin_memcpy(v, p, 16); }
+template <class E>
+__device__ __forceinline__ void store(E* p, const E (&v)[16 / sizeof(E)]) { __builtin_memcpy(p, v, 16); }
+
+// To the type of the result, from 32 bits in every kind of item: left to itself the compiler rounds some fp16 results straight from the product and sum, and
+// then a pair turned in place could differ by the last bit from the same pair turned into a new tensor.
+template <class E>
+__device__ __forceinline__ E rounded(float x) {
+  asm("" : "+v"(x));
+  return (E)x;
+}
+
+template <int T, bool ADJ>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   using E = typename Elem<T>::type;
-  using Vec = typename Bytes<sizeof(E) * VE>::type;
-  struct alignas(sizeof(E) * VE) Pack { E e[VE]; };
+  constexpr int VE = 16 / sizeof(E);
   extern __shared__ float2 lds_cs[];  // [tokens][pairs]
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n_tok = (int)(a.total - t0 < a.tokens ? a.total - t0 : a.tokens);
+  const int64_t b0 = t0 / a.rows;
+  const uint32_t l0 = (uint32_t)(t0 % a.rows), rows = (uint32_t)a.rows;  // l0 + tokens stays below 2^32
   for (int i = threadIdx.x; i < n_tok * a.pairs; i += 256) {
-    const int64_t t = t0 + i / a.pairs, b = t / a.rows, l = t % a.rows;
+    const uint32_t at_row = l0 + i / a.pairs;
+    const int64_t b = b0 + at_row / rows, l = at_row % rows;
     const int j = i % a.pairs;
     float2 cs;
     if (a.positions) {
@@ -86,66 +97,76 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   }
   __syncthreads();
   // work items of a token: for every head of q, then of k, the vectors that hold its pairs ("halves": a vector of x and the one of y that
-  // belongs to it), then the vectors that are only copied
-  const int rot_items = (ADJ ? 2 * a.pairs : a.pairs) / VE;
-  const int items = rot_items + (a.copy_rest ? (a.dim - 2 * a.pairs) / VE : 0);
+  // belongs to it; the last vector may reach back over the one before it), the pairs that fill no vector, and the same of what is only copied
+  const int items = a.rot_vecs + a.rot_ones + a.copy_vecs + a.copy_ones;
   const int per_token = items * (a.heads + a.kv_heads);
+  const int turned = ADJ ? 2 * a.pairs : a.pairs;  // elements that the vectors go over
   for (int i = threadIdx.x; i < n_tok * per_token; i += 256) {
     const int tok = i / per_token, rest = i - tok * per_token;
-    const int head = rest / items, it = rest - head * items;
-    const int64_t t = t0 + tok, b = t / a.rows, l = t % a.rows;
+    const int head = rest / items;
+    int it = rest - head * items;
+    const uint32_t at_row = l0 + tok;
+    const int64_t b = b0 + at_row / rows, l = at_row % rows;
     const bool is_k = head >= a.heads;
     const E* src = is_k ? reinterpret_cast<const E*>(a.k) + b * a.k_b + l * a.k_l + (head - a.heads) * a.k_h
                         : reinterpret_cast<const E*>(a.q) + b * a.q_b + l * a.q_l + head * a.q_h;
     E* dst = is_k ? reinterpret_cast<E*>(a.k_out) + b * a.ko_b + l * a.ko_l + (head - a.heads) * a.ko_h
                   : reinterpret_cast<E*>(a.q_out) + b * a.qo_b + l * a.qo_l + head * a.qo_h;
-    if (it >= rot_items) {
-      const int c = 2 * a.pairs + (it - rot_items) * VE;
-      *reinterpret_cast<Vec*>(dst + c) = *reinterpret_cast<const Vec*>(src + c);
-      continue;
-    }
     const float2* cs = lds_cs + tok * a.pairs;
-    if constexpr (ADJ) {
-      if constexpr (VE == 1) {  // one element at a time still needs its neighbour: the even one's item does both
-        if (it & 1) continue;
-        const float x = (float)src[it], y = (float)src[it + 1];
-        const float2 w = cs[it >> 1];
-        dst[it] = (E)__builtin_fmaf(x, w.x, -y * w.y);
-        dst[it + 1] = (E)__builtin_fmaf(y, w.x, x * w.y);
-      } else {
-        Pack v = __builtin_bit_cast(Pack, *reinterpret_cast<const Vec*>(src + it * VE));
+    if (it < a.rot_vecs) {
+      const int c = min(it * VE, turned - VE);
+      E x[VE], y[VE];
+      load(x, src + c);
+      if constexpr (ADJ) {
+        const float2* cw = cs + (c >> 1);
 #pragma unroll
         for (int e = 0; e < VE; e += 2) {
-          const float x = (float)v.e[e], y = (float)v.e[e + 1];
-          const float2 w = cs[(it * VE + e) >> 1];
-          v.e[e] = (E)__builtin_fmaf(x, w.x, -y * w.y);
-          v.e[e + 1] = (E)__builtin_fmaf(y, w.x, x * w.y);
+          const float2 w = cw[e / 2];
+          y[e] = rounded<E>(__builtin_fmaf((float)x[e], w.x, -(float)x[e + 1] * w.y));
+          y[e + 1] = rounded<E>(__builtin_fmaf((float)x[e + 1], w.x, (float)x[e] * w.y));
         }
-        *reinterpret_cast<Vec*>(dst + it * VE) = __builtin_bit_cast(Vec, v);
-      }
-    } else {
-      Pack vx = __builtin_bit_cast(Pack, *reinterpret_cast<const Vec*>(src + it * VE));
-      Pack vy = __builtin_bit_cast(Pack, *reinterpret_cast<const Vec*>(src + a.pairs + it * VE));
+        store(dst + c, y);
+      } else {
+        load(y, src + a.pairs + c);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float x = (float)vx.e[e], y = (float)vy.e[e];
-        const float2 w = cs[it * VE + e];
-        vx.e[e] = (E)__builtin_fmaf(x, w.x, -y * w.y);
-        vy.e[e] = (E)__builtin_fmaf(y, w.x, x * w.y);
+        for (int e = 0; e < VE; ++e) {
+          const float xe = (float)x[e], ye = (float)y[e];
+          const float2 w = cs[c + e];
+          x[e] = rounded<E>(__builtin_fmaf(xe, w.x, -ye * w.y));
+          y[e] = rounded<E>(__builtin_fmaf(ye, w.x, xe * w.y));
+        }
+        store(dst + c, x);
+        store(dst + a.pairs + c, y);
       }
-      *reinterpret_cast<Vec*>(dst + it * VE) = __builtin_bit_cast(Vec, vx);
-      *reinterpret_cast<Vec*>(dst + a.pairs + it * VE) = __builtin_bit_cast(Vec, vy);
+      continue;
+    }
+    it -= a.rot_vecs;
+    if (it < a.rot_ones) {
+      const int j = (ADJ ? a.rot_vecs * (VE / 2) : a.rot_vecs * VE) + it, cx = ADJ ? 2 * j : j, cy = ADJ ? cx + 1 : j + a.pairs;
+      const float x = (float)src[cx], y = (float)src[cy];
+      const float2 w = cs[j];
+      dst[cx] = rounded<E>(__builtin_fmaf(x, w.x, -y * w.y));
+      dst[cy] = rounded<E>(__builtin_fmaf(y, w.x, x * w.y));
+      continue;
+    }
+    it -= a.rot_ones;
+    const int c = 2 * a.pairs, n = a.dim - c;
+    if (it < a.copy_vecs) {
+      const int at = c + min(it * VE, n - VE);
+      E x[VE];
+      load(x, src + at);
+      store(dst + at, x);
+    } else {
+      const int at = c + it - a.copy_vecs;  // there are vectors or single elements, not both
+      dst[at] = src[at];
     }
   }
 }
 
 template <int T>
-void launch_rotary(const RotaryArgs& a, bool wide, bool adjacent, unsigned blocks, size_t lds, hipStream_t s) {
-  constexpr int VE = 16 / sizeof(typename Elem<T>::type);
-  if (wide && adjacent) hipLaunchKernelGGL((rotary_kernel<T, VE, true>), dim3(blocks), dim3(256), lds, s, a);
-  else if (wide) hipLaunchKernelGGL((rotary_kernel<T, VE, false>), dim3(blocks), dim3(256), lds, s, a);
-  else if (adjacent) hipLaunchKernelGGL((rotary_kernel<T, 1, true>), dim3(blocks), dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, 1, false>), dim3(blocks), dim3(256), lds, s, a);
+void launch_rotary(const RotaryArgs& a, bool adjacent, unsigned blocks, size_t lds, hipStream_t s) {
+  if (adjacent) hipLaunchKernelGGL((rotary_kernel<T, true>), dim3(blocks), dim3(256), lds, s, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, false>), dim3(blocks), dim3(256), lds, s, a);
 }
 
 }  // namespace
@@ -187,25 +208,30 @@ int mv_enc_rotary(int device, const mv_rotary* p, void* stream) {
   a.tab_b = p->table_batch, a.tab_l = p->table_row, a.tab_p = p->table_pair;
   a.scale = p->scale;
   a.batch = p->batch, a.rows = p->rows, a.heads = p->heads, a.kv_heads = p->kv_heads, a.dim = p->dim, a.pairs = p->pairs, a.total = total;
-  const bool in_place = (!p->heads || p->q == p->q_out) && (!p->kv_heads || p->k == p->k_out);
-  a.copy_rest = !in_place && 2 * p->pairs < p->dim;
+  const bool q_in_place = p->heads && p->q == p->q_out, k_in_place = p->kv_heads && p->k == p->k_out;
+  const bool copy = 2 * p->pairs < p->dim && ((p->heads && !q_in_place) || (p->kv_heads && !k_in_place));
 
-  // 16-byte vectors where every vector of pairs (and of the rest) starts at a multiple of 16 bytes; else element by element
   const int size = p->dtype == MV_F32 ? 4 : 2, ve = 16 / size;
-  int64_t strides = 0;
   uintptr_t ptrs = 0;
-  if (p->heads) strides |= a.q_b | a.q_l | a.q_h | a.qo_b | a.qo_l | a.qo_h, ptrs |= (uintptr_t)a.q | (uintptr_t)a.q_out;
-  if (p->kv_heads) strides |= a.k_b | a.k_l | a.k_h | a.ko_b | a.ko_l | a.ko_h, ptrs |= (uintptr_t)a.k | (uintptr_t)a.k_out;
+  if (p->heads) ptrs |= (uintptr_t)a.q | (uintptr_t)a.q_out;
+  if (p->kv_heads) ptrs |= (uintptr_t)a.k | (uintptr_t)a.k_out;
   if (ptrs & (size - 1)) {
     set_error("mv_enc_rotary: q and k must be aligned to their elements");
     return MV_ERR_INVALID;
   }
-  const bool wide = !(ptrs & 15) && strides % ve == 0 && (p->adjacent ? 2 * p->pairs : p->pairs) % ve == 0 && (!a.copy_rest || p->dim % ve == 0);
+  // The last vector reaches back over the one before it, which writes the same values twice; in place, where it could read what has been turned
+  // already, the pairs behind the last full vector go one by one.
+  const int turned = p->adjacent ? 2 * p->pairs : p->pairs, rest = copy ? p->dim - 2 * p->pairs : 0;
+  const bool reach_back = turned >= ve && !q_in_place && !k_in_place;
+  a.rot_vecs = reach_back ? (turned + ve - 1) / ve : turned / ve;
+  a.rot_ones = reach_back ? 0 : (turned - a.rot_vecs * ve) / (p->adjacent ? 2 : 1);
+  a.copy_vecs = rest >= ve ? (rest + ve - 1) / ve : 0;
+  a.copy_ones = rest >= ve ? 0 : rest;
 
-  // tokens of a block: enough to give every thread a vector or two, as few as that, so that small calls still spread over the card (8 pages of 1101
-  // tokens x 18 heads of 128, from memory: 18.3 us with 512 items a block, 22.2 with 256, 18.9 with 1024, 22.7 with 2048)
-  const int64_t vecs = std::max<int64_t>(1, (int64_t)(p->heads + p->kv_heads) * p->dim / (wide ? 2 * ve : 2));
-  int64_t tokens = std::max<int64_t>(1, 512 / vecs);
+  // tokens of a block: 1024 vectors, enough to give every thread a few, as few as that, so that small calls still spread over the card (8 pages of 1101
+  // tokens x 18 heads of 128, from memory: 18.3 us with 1024 vectors a block, 22.2 with 512, 18.9 with 2048, 22.7 with 4096)
+  const int64_t vectors = (p->adjacent ? 1 : 2) * a.rot_vecs + a.rot_ones + a.copy_vecs + a.copy_ones;
+  int64_t tokens = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, (p->heads + (int64_t)p->kv_heads) * vectors));
   tokens = std::min<int64_t>(tokens, std::max<int64_t>(1, 32768 / std::max<int64_t>(8, (int64_t)p->pairs * 8)));
   a.tokens = (int32_t)std::min<int64_t>(tokens, total);
   const int64_t blocks = (total + a.tokens - 1) / a.tokens;
@@ -216,9 +242,9 @@ int mv_enc_rotary(int device, const mv_rotary* p, void* stream) {
   const size_t lds = (size_t)std::max(1, a.tokens * a.pairs) * sizeof(float2);
   DeviceGuard g(device);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (p->dtype == MV_F32) launch_rotary<0>(a, wide, p->adjacent, (unsigned)blocks, lds, s);
-  else if (p->dtype == MV_BF16) launch_rotary<1>(a, wide, p->adjacent, (unsigned)blocks, lds, s);
-  else launch_rotary<2>(a, wide, p->adjacent, (unsigned)blocks, lds, s);
+  if (p->dtype == MV_F32) launch_rotary<0>(a, p->adjacent, (unsigned)blocks, lds, s);
+  else if (p->dtype == MV_BF16) launch_rotary<1>(a, p->adjacent, (unsigned)blocks, lds, s);
+  else launch_rotary<2>(a, p->adjacent, (unsigned)blocks, lds, s);
   MV_HIP(hipGetLastError());
   return MV_OK;
 }

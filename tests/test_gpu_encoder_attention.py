@@ -20,7 +20,8 @@ def ea():
     from morphik_core_amd import encoder_attention
 
     assert torch.cuda.is_available()
-    return encoder_attention
+    yield encoder_attention
+    torch.cuda.empty_cache()  # the tests behind fill the card with their slabs
 
 
 def gen(seed):
@@ -388,6 +389,29 @@ def test_rotation_of_every_width_type_and_layout(ea, dtype, pairing, dim, sectio
         assert none is None and none2 is None and torch.equal(only_q, got[0]) and torch.equal(only_k, got[1])
         a, b = ea.rotary(q, k, pos, table, in_place=True)
         assert a is q and b is k and torch.equal(q, got[0]) and torch.equal(k, got[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("pairing", ["halves", "adjacent"])
+@pytest.mark.parametrize("dim,pairs", [(72, 36), (72, 13), (40, 20), (23, 11), (17, 1), (9, 4), (24, 12), (130, 65)])
+def test_rotation_at_any_alignment_leaves_its_neighbours(ea, dtype, pairing, dim, pairs):
+    """Heads that start anywhere in 16 bytes, three elements between heads, five between rows: the elements between stay, in place gives the same bits."""
+    g, heads, rows = gen(dim + pairs), 3, 41
+    table = ea.RotaryTable.with_sections(dim, [pairs], rot_dim=2 * pairs, pairing=pairing)
+    pos = torch.randint(0, 1000, (1, 1, rows), generator=g, device="cuda")
+    cos, sin = angles(pos, table)
+    for offset in (0, 1, 2, 5):
+        row = heads * (dim + 3) + 5
+        flat = torch.randn(offset + rows * row, generator=g, device="cuda").to(DT[dtype])
+        before = flat.clone()
+        q = flat.as_strided((1, rows, heads, dim), (rows * row, row, dim + 3, 1), offset)
+        got = ea.rotary(q, None, pos, table)[0]
+        check(got, *rotary_oracle(q, cos, sin, pairing))
+        assert torch.equal(flat, before)
+        ea.rotary(q, None, pos, table, in_place=True)
+        assert torch.equal(q, got)
+        before.as_strided(q.shape, q.stride(), offset).copy_(got)
+        assert torch.equal(flat, before)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])

@@ -62,16 +62,17 @@ def _dtype_code(torch, dtype, what: str, fp32: bool) -> int:
 
 def _device_index(torch, what: str, *tensors: Any) -> int:
     """All on one GPU, none that autograd would follow.  -> its index"""
-    device = tensors[0].device
-    if device.type != "cuda":
+    index = tensors[0].get_device()
+    if index < 0:
         raise ValueError(f"{what}: tensors must be on a GPU (there is no CPU path)")
-    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t.device != device:
-            raise ValueError(f"{what}: tensors on different devices ({device}, {t.device})")
-        if grad and t.requires_grad:
-            raise ValueError(f"{what}: has no gradient (run it under torch.inference_mode() or torch.no_grad())")
-    return device.index
+        if t.get_device() != index:
+            raise ValueError(f"{what}: tensors on different devices ({tensors[0].device}, {t.device})")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError(f"{what}: has no gradient (run it under torch.inference_mode() or torch.no_grad())")
+    return index
 
 
 def _stream(torch, index: int) -> int:
@@ -370,6 +371,15 @@ def _workspace_bytes(index: int, *sizes: int) -> int:
     return int(n)
 
 
+def _steps(what: str, name: str, t: Any) -> Tuple[int, ...]:
+    """Strides of batch, rows and heads; a dimension of one entry has none."""
+    st = t.stride()
+    steps = tuple(0 if n == 1 else x for n, x in zip(t.shape, st[:3]))
+    if t.numel() and (st[3] != 1 or t.data_ptr() & 15 or (steps[0] | steps[1] | steps[2]) & 7):
+        raise ValueError(f"{what}: {name} must be 16-byte aligned, strides multiples of 8, the elements of a head side by side")
+    return steps
+
+
 def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = False, scale: Optional[float] = None, softcap: float = 0.0) -> Any:
     """Softmax attention of q [batch, rows, heads, dim] over k, v [batch, keys, kv_heads, dim] (or [rows, heads, dim] of packed documents), heads
     a multiple of kv_heads.  key_ranges int32 [batch or 1, rows, 2]: row i sees the keys [lo, hi), cut to what there is; an empty range gives
@@ -382,7 +392,8 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
     code = _dtype_code(torch, q.dtype, what, fp32=False)
     if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError(f"{what}: q, k and v differ in type ({q.dtype}, {k.dtype}, {v.dtype})")
-    q, k, v = _heads4(q, what, "q"), _heads4(k, what, "k"), _heads4(v, what, "v")
+    if len(shape) != 4 or k.dim() != 4 or v.dim() != 4:
+        q, k, v = _heads4(q, what, "q"), _heads4(k, what, "k"), _heads4(v, what, "v")
     batch, rows, heads, dim = q.shape
     k_shape = k.shape
     k_batch, keys, kv_heads, k_dim = k_shape
@@ -397,25 +408,22 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
         raise ValueError(f"{what}: scale must be positive and finite")
     if not (softcap >= 0 and math.isfinite(softcap)):
         raise ValueError(f"{what}: softcap must not be negative (0: no cap)")
-    pointers, strides = [], []
-    for name, t, sizes in (("q", q, q.shape), ("k", k, k_shape), ("v", v, k_shape)):
-        st, at = t.stride(), t.data_ptr()
-        if (st[3] != 1 or at & 15 or (st[0] | st[1] | st[2]) & 7) and t.numel():
-            # a dimension of one entry has no step
-            st = tuple(0 if n == 1 else x for n, x in zip(sizes, st[:3])) + (st[3],)
-            if st[3] != 1 or at & 15 or (st[0] | st[1] | st[2]) & 7:
-                raise ValueError(f"{what}: {name} must be 16-byte aligned, strides multiples of 8, the elements of a head side by side")
-        pointers.append(at)
-        strides += st[:3]
+    at_q, at_k, at_v, st_q, st_k, st_v = q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(), k.stride(), v.stride()
+    q0, q1, q2, q3 = st_q
+    k0, k1, k2, k3 = st_k
+    v0, v1, v2, v3 = st_v
+    if (at_q | at_k | at_v) & 15 or (q0 | q1 | q2 | k0 | k1 | k2 | v0 | v1 | v2) & 7 or not q3 == k3 == v3 == 1:
+        (q0, q1, q2), (k0, k1, k2), (v0, v1, v2) = (_steps(what, name, t) for name, t in (("q", q), ("k", k), ("v", v)))
     if key_ranges is not None:
         if causal:
             raise ValueError(f"{what}: causal goes without key_ranges (padded_ranges(..., prefix=0) makes causal ones)")
-        if key_ranges.dtype is not torch.int32 or key_ranges.dim() != 3 or key_ranges.shape[0] not in (1, batch) or tuple(key_ranges.shape[1:]) != (rows, 2):
+        r_shape = key_ranges.shape
+        if key_ranges.dtype is not torch.int32 or len(r_shape) != 3 or r_shape[0] not in (1, batch) or r_shape[1] != rows or r_shape[2] != 2:
             raise ValueError(f"{what}: key_ranges must be int32 [{batch} or 1, {rows}, 2], not {key_ranges.dtype} {tuple(key_ranges.shape)}")
         index = _device_index(torch, what, q, k, v, key_ranges)
         if not key_ranges.is_contiguous() or key_ranges.data_ptr() & 7:
             key_ranges = key_ranges.clone(memory_format=torch.contiguous_format)
-        ranges, ranges_batch = key_ranges.data_ptr(), 0 if key_ranges.shape[0] == 1 else 2 * rows
+        ranges, ranges_batch = key_ranges.data_ptr(), 0 if r_shape[0] == 1 else 2 * rows
     else:
         index = _device_index(torch, what, q, k, v)
         ranges = ranges_batch = 0
@@ -423,7 +431,7 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
     if batch and rows:
         need = _workspace_bytes(index, batch, rows, keys, heads, kv_heads, dim)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # torch's own reuse rules keep it this call's on this stream
-        packed = _PACK_ATTN.pack(*pointers, out.data_ptr(), ranges, *strides, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, int(causal), scale, softcap)
+        packed = _PACK_ATTN.pack(at_q, at_k, at_v, out.data_ptr(), ranges, q0, q1, q2, k0, k1, k2, v0, v1, v2, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, int(causal), scale, softcap)
         _lib.check(_lib.lib().mv_enc_attention(index, packed, _stream(torch, index)))
     return out if len(shape) == 4 else out.view(shape)
 

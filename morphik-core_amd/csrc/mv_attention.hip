@@ -48,6 +48,9 @@ constexpr int built_kc(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 
 constexpr int kMatrix = 0x008, kDsRead = 0x100;  // classes of __builtin_amdgcn_sched_group_barrier
 constexpr float kRescale = 8.f;                // running maxima move only when a score passes them by 2^8: the weights stay <= 256
 
+// In place of a run's sum of weights: the row is not in pieces and done, the row sees nothing of the run
+constexpr float kDone = -1.f, kUnseen = -2.f;
+
 constexpr int64_t kMaxRowStride = 1 << 23;    // elements: a tile's byte offsets stay below 2^31
 
 struct AttnArgs {
@@ -263,10 +266,10 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
   if (k_lo >= k_hi) k_lo = k_hi = 0;  // no row of the block sees anything: positions stay far from the end of 32 bits
   if (partial) {
     const int tiles = (k_hi - k_lo + BK - 1) / BK;
-    const int pieces = max(min(a.splits, tiles / 2), 1);  // short ranges stay in one piece, and are told apart by a sum of -1
+    const int pieces = max(min(a.splits, tiles / 2), 1);  // short ranges stay in one piece
     if (pieces == 1) {
       if (split) return;
-      if (live && half == 0) *reinterpret_cast<float2*>(partial + (wave * kWaveRows + lane) * (a.dim + 4) + a.dim) = make_float2(-INFINITY, -1.f);
+      if (live && half == 0) *reinterpret_cast<float2*>(partial + (wave * kWaveRows + lane) * (a.dim + 4) + a.dim) = make_float2(-INFINITY, kDone);
       partial = nullptr;
     } else {
       const int share = (tiles + pieces - 1) / pieces * BK;  // whole tiles
@@ -455,7 +458,7 @@ __global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_p
           *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = nothing ? u32x2{0, 0} : w;
         }
   } else if (live_e) {
-    if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
+    if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, kUnseen) : make_float2(m, l);
     if (!nothing) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -494,25 +497,29 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
   const bool live = in_tile < stored && r < all;  // of the whole group of W waves
   const int64_t step = (int64_t)stored * (a.dim + 4);
   const float* src = a.partial + (int64_t)cut * a.splits * step + (int64_t)(live ? in_tile : 0) * (a.dim + 4);
-  if (src[a.dim + 1] == -1.f) return;  // not in pieces after all: the row is done (W waves see the same row, and end together)
+  if (src[a.dim + 1] == kDone) return;  // not in pieces after all: the row is done (W waves see the same row, and end together)
   float m = -INFINITY, l = 0.f;
+  bool seen = false;
   f32x4 o = {};
   if (live) {
     for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, src[s * step + a.dim]);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     for (int s0 = 0; s0 < a.splits; s0 += 64) {
-      float w = 0.f;  // of run s0 + lane; 0 where the row sees nothing of it (its sums were never written)
+      float w = -1.f;  // of run s0 + lane; below 0 where the row sees nothing of it (its sums were never written)
       if (s0 + lane < a.splits) {
         const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + a.dim);
-        if (ml.y != 0.f) w = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
-        l = __builtin_fmaf(ml.y, w, l);
+        if (ml.y != kUnseen) {
+          seen = true;
+          w = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+          l = __builtin_fmaf(ml.y, w, l);
+        }
       }
       const int n = min(64, a.splits - s0);
 #pragma unroll 8
       for (int i = wave % W; i < n; i += W) {
         const float wi = __shfl(w, i);
-        const f32x4 part = lane * 4 < a.dim && wi != 0.f ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
+        const f32x4 part = lane * 4 < a.dim && !(wi < 0.f) ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(part[e], wi, o[e]);
       }
@@ -527,7 +534,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
 #pragma unroll
     for (int i = 1; i < W; ++i) o += lds_o[wave + i][lane];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = __any(seen) ? 1.f / l : 0.f;  // a row whose scores are all -infinity is seen: not a number, as in one piece
   if (live && lane * 4 < a.dim) {
     const int64_t pos = r / a.group, head = hk * a.group + r % a.group;
     *reinterpret_cast<u32x2*>(a.out + b * a.o_b + pos * a.o_l + head * a.o_h + lane * 4) =
@@ -676,7 +683,8 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
     set_error("mv_enc_attention: pointers must be set and 16-byte aligned, strides multiples of 8 elements");
     return MV_ERR_INVALID;
   }
-  if (p->k_row < 0 || p->k_row > kMaxRowStride || p->v_row < 0 || p->v_row > kMaxRowStride) {
+  const int64_t k_row = p->keys > 1 ? p->k_row : 0, v_row = p->keys > 1 ? p->v_row : 0;  // one key has no step
+  if (k_row < 0 || k_row > kMaxRowStride || v_row < 0 || v_row > kMaxRowStride) {
     set_error("mv_enc_attention: rows of k or v more than %lld elements apart", (long long)kMaxRowStride);
     return MV_ERR_INVALID;
   }
@@ -688,8 +696,8 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   a.ranges = reinterpret_cast<const int32_t*>(p->ranges);
   a.range_b = p->ranges_batch;
   a.q_b = p->q_batch, a.q_l = p->q_row, a.q_h = p->q_head;
-  a.k_b = p->k_batch, a.k_l = p->k_row, a.k_h = p->k_head;
-  a.v_b = p->v_batch, a.v_l = p->v_row, a.v_h = p->v_head;
+  a.k_b = p->k_batch, a.k_l = k_row, a.k_h = p->k_head;
+  a.v_b = p->v_batch, a.v_l = v_row, a.v_h = p->v_head;
   a.o_h = p->dim, a.o_l = (int64_t)p->heads * p->dim, a.o_b = a.o_l * p->rows;
   a.rows = p->rows, a.keys = p->keys, a.kv_heads = p->kv_heads, a.group = p->heads / p->kv_heads, a.dim = p->dim, a.causal = p->causal && !p->ranges;
   if (p->softcap > 0.f) {
@@ -697,6 +705,10 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
     a.cap = p->softcap * kLog2e;
   } else {
     a.qk = p->scale * kLog2e;
+  }
+  if (!(a.qk > 0.f) || !std::isfinite(a.qk) || !std::isfinite(a.cap)) {
+    set_error("mv_enc_attention: scale or scale / softcap leaves 32 bits");
+    return MV_ERR_INVALID;
   }
   const int64_t tall = (int64_t)p->rows * a.group;  // rows of one K/V head
   const Plan pl = plan(p->batch, p->rows, p->keys, p->heads, p->kv_heads, p->dim, cu_count(device));

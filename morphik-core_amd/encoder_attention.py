@@ -29,6 +29,7 @@ from typing import Any, Dict, Optional, Sequence, Tuple
 from . import _lib
 
 _PAIRINGS = ("halves", "adjacent")
+_FP32_MAX = 2.0**128 - 2.0**104
 _FORMATS = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
 
 
@@ -115,7 +116,7 @@ class RotaryTable:
             raise ValueError(f"RotaryTable: {pairs} pairs do not fit a head of {head_dim} (at most 4096)")
         if pairing not in _PAIRINGS:
             raise ValueError(f"RotaryTable: pairing {pairing!r} (one of {_PAIRINGS})")
-        if not math.isfinite(scale):
+        if not abs(scale) < _FP32_MAX:
             raise ValueError("RotaryTable: scale must be finite")
         self.head_dim, self.pairs, self.pairing, self.scale = int(head_dim), pairs, pairing, float(scale)
         self.axes = int(host.max()) + 1 if pairs else 0  # axes that positions must have at least
@@ -383,8 +384,9 @@ def _steps(what: str, name: str, t: Any) -> Tuple[int, ...]:
 def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = False, scale: Optional[float] = None, softcap: float = 0.0) -> Any:
     """Softmax attention of q [batch, rows, heads, dim] over k, v [batch, keys, kv_heads, dim] (or [rows, heads, dim] of packed documents), heads
     a multiple of kv_heads.  key_ranges int32 [batch or 1, rows, 2]: row i sees the keys [lo, hi), cut to what there is; an empty range gives
-    zeros; None: every key, or with `causal` those up to the row itself (the last row stands at the last key).  scale defaults to dim ** -0.5; softcap c > 0 caps scores to c * tanh(score / c).  bfloat16 or float16; dim a multiple
-    of 8 up to 256; any strides that are multiples of 8 with the elements of a head side by side, 16-byte aligned.
+    zeros; None: every key, or with `causal` those up to the row itself (the last row stands at the last key).  scale defaults to dim ** -0.5; softcap
+    c > 0 caps scores to c * tanh(score / c).  bfloat16 or float16; dim a multiple of 8 up to 256; any strides that are multiples of 8 with the elements
+    of a head side by side, 16-byte aligned.
     -> new contiguous tensor of q's shape."""
     torch = _torch()
     what = "attention"
@@ -404,9 +406,9 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
     if dim % 8 or not 8 <= dim <= 256:
         raise ValueError(f"{what}: heads of {dim} (multiples of 8 up to 256)")
     scale = dim**-0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if not 0 < scale < _FP32_MAX:
         raise ValueError(f"{what}: scale must be positive and finite")
-    if not (softcap >= 0 and math.isfinite(softcap)):
+    if not 0 <= softcap < _FP32_MAX:
         raise ValueError(f"{what}: softcap must not be negative (0: no cap)")
     at_q, at_k, at_v, st_q, st_k, st_v = q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(), k.stride(), v.stride()
     q0, q1, q2, q3 = st_q
@@ -431,7 +433,8 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
     if batch and rows:
         need = _workspace_bytes(index, batch, rows, keys, heads, kv_heads, dim)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # torch's own reuse rules keep it this call's on this stream
-        packed = _PACK_ATTN.pack(at_q, at_k, at_v, out.data_ptr(), ranges, q0, q1, q2, k0, k1, k2, v0, v1, v2, ranges_batch, work.data_ptr() if need else 0, need, code, batch, rows, keys, heads, kv_heads, dim, int(causal), scale, softcap)
+        packed = _PACK_ATTN.pack(at_q, at_k, at_v, out.data_ptr(), ranges, q0, q1, q2, k0, k1, k2, v0, v1, v2, ranges_batch, work.data_ptr() if need else 0, need,
+                                 code, batch, rows, keys, heads, kv_heads, dim, int(causal), scale, softcap)
         _lib.check(_lib.lib().mv_enc_attention(index, packed, _stream(torch, index)))
     return out if len(shape) == 4 else out.view(shape)
 

@@ -225,6 +225,19 @@ def test_the_c_entries_refuse_bad_structs_before_any_launch():
     assert L.mv_enc_document_ranges(0, None, 1, None, -1, 0, None, None) == 0
 
 
+def test_scales_that_leave_32_bits_are_refused():
+    q, k, v = qkv()
+    with pytest.raises(ValueError, match="scale"):
+        ea.attention(q, k, v, scale=1e39)
+    with pytest.raises(ValueError, match="softcap"):
+        ea.attention(q, k, v, softcap=1e39)
+    with pytest.raises(ValueError, match="finite"):
+        ea.RotaryTable([1.0], head_dim=16, scale=1e39, device="cpu")
+    for scale, cap in ((3e38, 0.0), (3e38, 1e-3), (1e-30, 1e30), (1.0, 3e38)):  # in range themselves, but not scale * log2(e), scale / cap or cap * log2(e)
+        p = _lib.AttnC(q=16, k=16, v=16, out=16, dtype=_lib.MV_BF16, batch=1, rows=1, keys=1, heads=2, kv_heads=1, dim=16, scale=scale, softcap=cap)
+        assert _lib.lib().mv_enc_attention(0, C.byref(p), None) == -1 and "32 bits" in _lib.lib().mv_last_error().decode()
+
+
 def test_the_structs_are_laid_out_as_the_header_declares_them(tmp_path):
     """sizeof and the last field's offset, from a C compiler over include/mvmaxsim.h."""
     src = tmp_path / "s.c"

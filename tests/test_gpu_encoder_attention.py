@@ -240,6 +240,26 @@ def test_scores_of_extreme_size(ea):
     check(ea.attention(q, k, v, scale=3.0), *oracle(q, k, v, scale=3.0))
 
 
+@pytest.mark.parametrize("rows,keys", [(3, 40), (40, 70), (1, 3000), (4, 3000)])
+@pytest.mark.parametrize("dim", [40, 128])
+def test_scores_of_minus_infinity(ea, dim, rows, keys):
+    """Keys whose scores are -infinity weigh nothing; a row that sees no other key is 0 / 0 by the formula, whether or not it is cut along the keys; a row
+    that sees no key at all is zero."""
+    g = gen(dim + keys)
+    q, k, v = (make(g, 1, n, h, dim, DT["bf16"], "split") for n, h in ((rows, 2), (keys, 1), (keys, 1)))
+    q[..., 0] = 1.0
+    half = keys // 2
+    k[:, :half, :, 0] = -math.inf
+    cut = torch.tensor([half, keys], dtype=torch.int32, device="cuda").expand(1, rows, 2).contiguous()
+    check(ea.attention(q, k, v), *oracle(q, k, v, cut))
+    ranges = torch.tensor([0, half], dtype=torch.int32, device="cuda").repeat(1, rows, 1)
+    ranges[:, 0] = half
+    got = ea.attention(q, k, v, key_ranges=ranges)
+    assert not bool(got[:, 0].any()) and bool(got[:, 1:].isnan().all())
+    k[:, :, :, 0] = -math.inf
+    assert bool(ea.attention(q, k, v).isnan().all())
+
+
 def test_sizes_of_nothing(ea):
     q, k, v = (make(gen(1), 2, 5, h, 16, DT["fp16"], "split") for h in (4, 2, 2))
     assert not bool(ea.attention(q, k[:, :0], v[:, :0]).any())
@@ -256,6 +276,14 @@ def test_strides_of_one_entry_do_not_matter(ea):
     q2 = odd.as_strided((1, 9, 1, 16), (9 * 147 + 1, 16, 7, 1))
     q2.copy_(q)
     assert torch.equal(ea.attention(q2, k, v), ea.attention(q, k, v))
+
+
+def test_one_key_has_no_step(ea):
+    """Rows of k and v may be at most 2^23 elements apart, but one row is apart from nothing."""
+    g = gen(6)
+    q, k, v = (make(g, 1, n, 1, 16, DT["bf16"], "split") for n in (9, 1, 1))
+    far = (1 << 25, 1 << 24, 16, 1)
+    assert torch.equal(ea.attention(q, k.as_strided(k.shape, far), v.as_strided(v.shape, far)), v.expand(1, 9, 1, 16))
 
 
 def test_offsets_past_32_bits(ea):

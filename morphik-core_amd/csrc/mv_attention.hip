@@ -42,7 +42,11 @@ constexpr int kXcds = 8;
 constexpr int tile_keys(int kc) { return kc > 8 ? 32 : 64; }
 constexpr int waves_per_simd(int kc) { return kc <= 4 ? 4 : 2; }
 constexpr int block_waves(int kc) { return kc == 5 || kc == 6 ? 4 : 8; }
-constexpr int block_rows(int kc) { return block_waves(kc) * kWaveRows; }
+constexpr int blocks_per_cu(int kc, int waves) {  // by registers, by the 160 KB of LDS (tiles of K and V twice, 2 KB of ranges)
+  const int by_waves = waves_per_simd(kc) * 4 / waves, by_lds = 160 * 1024 / (2 * tile_keys(kc) * (2 * kc + (kc + 1) / 2 * 4) * 16 + 2048);
+  return by_waves < by_lds ? by_waves : by_lds;
+}
+constexpr int kFewWaves = 2;  // of a block of a short call: see few_waves()
 // The widths that are built: a head takes the next wider one
 constexpr int built_kc(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : dim <= 128 ? 8 : dim <= 192 ? 12 : 16; }
 constexpr int kMatrix = 0x008, kDsRead = 0x100;  // classes of __builtin_amdgcn_sched_group_barrier
@@ -179,10 +183,10 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // K/V head 133 us (1.03), 8464 rows of 16 heads of 80 444 us (0.83; the 16-column and 32-column steps round 80 up to 80 and 96).  Tried and not kept: two
 // groups of waves half a tile apart (289 us at 128), the weights of 32 keys beside the products of the next 32 (292), 64 rows a wave
 // (289, and 209 at 256), wave priorities (no change).
-template <bool BF16, int KC, bool CAP>
-__global__ __launch_bounds__(block_waves(KC) * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(KC), waves_per_simd(KC)))) void attention_kernel(
+template <bool BF16, int KC, bool CAP, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(KC), waves_per_simd(KC)))) void attention_kernel(
     const AttnArgs a) {
-  constexpr int kWaves = block_waves(KC), kBlockRows = block_rows(KC);
+  constexpr int kBlockRows = kWaves * kWaveRows;
   constexpr int BK = tile_keys(KC);
   constexpr int DT = (KC + 1) / 2;             // 32-column tiles of the output; KC: 16-column steps of q.k
   constexpr int CH = 2 * KC;                   // 16-byte chunks of a row
@@ -553,25 +557,37 @@ __global__ void zero_rows_kernel(uint32_t* out, int64_t words) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) out[i] = 0;
 }
 
-// How the tiles of a call are dealt out.  A card takes waves_per_simd waves a SIMD at once; the tiles of the last, partly filled round are cut into
+// How the tiles of a call are dealt out.  A card takes blocks_per_cu a CU at once; the tiles of the last, partly filled round are cut into
 // runs of keys, as many as fill it, where what that saves (a tile takes about kTileUs per tile of keys in a filled CU) is more than writing,
 // reading and joining the runs' 32-bit sums costs (kJoinUs for the launch, kJoinBytesPerUs).
 struct Plan {
-  int64_t blocks, full, cut, splits, bytes;
+  int64_t waves, block_rows, blocks, full, cut, splits, bytes;
 };
+// Where eight-wave blocks would leave most of the card idle, blocks of two waves spread the rows over four times the CUs: where all of them fit at once and
+// the keys are few enough not to be cut along instead (us, bf16: 20 rows x 8 heads of 256 12.0 -> 7.9, 32 x 39 rows x 12 of 128 9.9 -> 7.2, 4 x 256 x 8 of
+// 256 26.2 -> 18.0, 4 x 500 39.3 -> 29.7, 2 x 500 x 12 of 128 20.0 -> 14.2; 1030 x 8 of 256, 33 tiles of keys, 43.1 -> 52.3, 1101 x 12 of 128, 18 tiles,
+// 35.9 -> 39.5, heads of 192, 25 tiles, 33.2 -> 30.4).  Rows that fill one block either way gain little (16 x 60 x 16 of 64 6.1 -> 5.6) and are better cut (40 x 1 row of 16 heads over 500 keys
+// 12.5 -> 14.9); heads of 72 ... 96, in four waves otherwise, lose (600 x 16 of 80 21.7 -> 23.5).
+bool few_waves(int64_t all, int64_t keys, int64_t problems, int kc, int64_t cus) {
+  constexpr int kRows = kFewWaves * kWaveRows;
+  return block_waves(kc) == 8 && keys <= (all > kRows ? 16 : 2) * tile_keys(kc) && (all + kRows - 1) / kRows * problems <= 2 * cus;
+}
 constexpr double kTileUs = 2.3, kJoinUs = 4.0, kJoinBytesPerUs = 4e6;
 
 Plan plan(int64_t batch, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, int64_t cus) {
   const int kc = built_kc((int)dim);
-  const int64_t all = rows * (heads / kv_heads), slots = cus * waves_per_simd(kc) * 4 / block_waves(kc);
+  const int64_t all = rows * (heads / kv_heads);
   Plan p = {};
-  p.blocks = (all + block_rows(kc) - 1) / block_rows(kc) * kv_heads * batch;
+  p.waves = few_waves(all, keys, kv_heads * batch, kc, cus) ? kFewWaves : block_waves(kc);
+  p.block_rows = p.waves * kWaveRows;
+  const int64_t slots = cus * blocks_per_cu(kc, (int)p.waves);
+  p.blocks = (all + p.block_rows - 1) / p.block_rows * kv_heads * batch;
   p.full = p.blocks / slots * slots;
   p.cut = p.blocks - p.full;
   p.splits = 1;
   if (p.cut == 0) return p;
   const int64_t key_tiles = (keys + tile_keys(kc) - 1) / tile_keys(kc);
-  const int64_t piece = std::min<int64_t>(block_rows(kc), all) * (dim + 4) * 4;
+  const int64_t piece = std::min<int64_t>(p.block_rows, all) * (dim + 4) * 4;
   // t(n) = key_tiles / n * kTileUs + kJoinUs + n * moved: least at n = sqrt(key_tiles * kTileUs / moved), then evened out to whole tiles
   const double moved = 2.0 * p.cut * piece / kJoinBytesPerUs;
   int64_t n = (int64_t)std::sqrt(key_tiles * kTileUs / moved);
@@ -597,7 +613,14 @@ int cu_count(int device) {
 
 template <bool BF16, int KC, bool CAP>
 void launch_attention(const AttnArgs& a, int64_t blocks, hipStream_t s) {
-  hipLaunchKernelGGL((attention_kernel<BF16, KC, CAP>), dim3((unsigned)blocks), dim3(block_waves(KC) * 64), 0, s, a);
+  constexpr int kMany = block_waves(KC);
+  if constexpr (kMany == 8) {
+    if (a.block_rows == kFewWaves * kWaveRows) {
+      hipLaunchKernelGGL((attention_kernel<BF16, KC, CAP, kFewWaves>), dim3((unsigned)blocks), dim3(kFewWaves * 64), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((attention_kernel<BF16, KC, CAP, kMany>), dim3((unsigned)blocks), dim3(kMany * 64), 0, s, a);
 }
 
 template <bool BF16, bool CAP>
@@ -721,7 +744,7 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
     set_error("mv_enc_attention: needs a 16-byte aligned workspace of %lld bytes (mv_enc_attention_workspace_bytes)", (long long)pl.bytes);
     return MV_ERR_INVALID;
   }
-  a.block_rows = block_rows(built_kc(p->dim));
+  a.block_rows = (int32_t)pl.block_rows;
   a.tiles = (int32_t)((tall + a.block_rows - 1) / a.block_rows);
   a.full = (int32_t)pl.full, a.splits = (int32_t)pl.splits;
   a.partial = reinterpret_cast<float*>(p->workspace);

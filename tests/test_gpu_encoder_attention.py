@@ -139,6 +139,22 @@ def test_few_rows_over_many_keys(ea, rows, keys, dtype):
         check(ea.attention(q, k, v, key_ranges=r), *oracle(q, k, v, r))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [16, 64, 80, 104, 128, 200, 256])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_small_and_large_blocks_of_every_width(ea, dtype, dim, softcap):
+    """Short calls (rows spread over more, smaller blocks, with and without a cut along the keys), long keys, and more short problems than the card holds."""
+    g = gen(dim + 1)
+    for batch, rows, keys, heads, kv in ((1, 20, 500, 8, 1), (2, 130, 480, 2, 2), (2, 500, 500, 6, 1), (1, 300, 1100, 6, 2), (300, 70, 40, 2, 2)):
+        q, k, v = (make(g, batch, n, h, dim, DT[dtype], "heads", x) for n, h, x in ((rows, heads, 2.0), (keys, kv, 1.0), (keys, kv, 1.0)))
+        check(ea.attention(q, k, v, softcap=softcap), *oracle(q, k, v, softcap=softcap), what=(rows, keys, "all"))
+        r = some_ranges(g, batch, rows, keys)
+        check(ea.attention(q, k, v, key_ranges=r, softcap=softcap), *oracle(q, k, v, r, softcap=softcap), what=(rows, keys, "ranges"))
+        last = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+        r = ea.padded_ranges(last // 5, last - 3, rows, prefix=0, row_offset=max(keys - rows, 0))
+        check(ea.attention(q, k, v, key_ranges=r, softcap=softcap), *oracle(q, k, v, r, softcap=softcap), what=(rows, keys, "causal"))
+
+
 @pytest.mark.parametrize("dim", [64, 80, 256])
 def test_masks_of_the_encoders(ea, dim):
     """Causal, prefix and two-sided padding on either side; packed documents of one to many rows, some of none; one range row for a whole batch."""

@@ -166,6 +166,7 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float first_lane(float x) { return __int_as_float(uniform(__float_as_int(x))); }
 
 // One block: 32 rows a wave against the keys that any of them sees, in tiles of BK keys staged through LDS.
 //
@@ -483,11 +484,13 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
   }
 }
 
-// Joins the runs of keys of the cut tiles: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A wave's lanes take the runs' weights first, so
-// that the loads of the sums do not wait for one another; W waves share a row (every W-th run each), added up in their order.
+// Joins the runs of keys of the cut tiles: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, join_runs of a wave at a time with the maximum moving as
+// in the loop above.  W waves share a row (every W-th run each), added up in their order.  Bound by latency: what a run left lies in another XCD's L2 or
+// behind it, so all loads of a round are sent for before anything is waited for (3 x 1 row of 16 heads over 16001 keys: 4.5 us; one round trip after the other 6.8).
+constexpr int join_runs(int w) { return w == 1 ? 8 : 16; }
 template <bool BF16, int W>
 __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
-  constexpr int kRows = 4 / W;  // of a block
+  constexpr int kRows = 4 / W, kRuns = join_runs(W);  // rows of a block, runs of a wave in a round
   __shared__ f32x4 lds_o[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t all = (int64_t)a.rows * a.group;
@@ -501,36 +504,46 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
   const bool live = in_tile < stored && r < all;  // of the whole group of W waves
   const int64_t step = (int64_t)stored * (a.dim + 4);
   const float* src = a.partial + (int64_t)cut * a.splits * step + (int64_t)(live ? in_tile : 0) * (a.dim + 4);
-  if (src[a.dim + 1] == kDone) return;  // not in pieces after all: the row is done (W waves see the same row, and end together)
   float m = -INFINITY, l = 0.f;
-  bool seen = false;
+  bool seen = false, done = false;
   f32x4 o = {};
-  if (live) {
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, src[s * step + a.dim]);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-    for (int s0 = 0; s0 < a.splits; s0 += 64) {
-      float w = -1.f;  // of run s0 + lane; below 0 where the row sees nothing of it (its sums were never written)
-      if (s0 + lane < a.splits) {
-        const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + a.dim);
-        if (ml.y != kUnseen) {
-          seen = true;
-          w = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
-          l = __builtin_fmaf(ml.y, w, l);
-        }
-      }
-      const int n = min(64, a.splits - s0);
-#pragma unroll 8
-      for (int i = wave % W; i < n; i += W) {
-        const float wi = __shfl(w, i);
-        const f32x4 part = lane * 4 < a.dim && !(wi < 0.f) ? *reinterpret_cast<const f32x4*>(src + (s0 + i) * step + lane * 4) : f32x4{};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(part[e], wi, o[e]);
-      }
+  const int own = uniform(wave % W), splits = live ? a.splits : 0;
+  for (int s0 = 0; s0 < splits; s0 += kRuns * W) {
+    float2 ml = make_float2(-INFINITY, kUnseen);  // of run s0 + lane
+    if (lane < kRuns * W && s0 + lane < splits) ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + a.dim);
+    if constexpr (W == 1) {  // not in pieces after all: the row is done, and where there are many rows their sums are not worth sending for
+      if (s0 == 0 && first_lane(ml.y) == kDone) return;
     }
+    f32x4 part[kRuns];
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+    for (int i = 0; i < kRuns; ++i) {
+      part[i] = f32x4{};
+      if (s0 + i * W + own < splits && lane * 4 < a.dim) part[i] = *reinterpret_cast<const f32x4*>(src + (s0 + i * W + own) * step + lane * 4);
+    }
+    if (s0 == 0) done = first_lane(ml.y) == kDone;
+    float top = ml.x;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float m2 = fmaxf(m, top), alpha = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m - m2);
+    // below 0 where the row sees nothing of the run (its sums were never written)
+    const float w = ml.y == kUnseen ? -1.f : m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m2);
+    m = m2;
+    l *= alpha;
+    if (!(w < 0.f)) {
+      seen = true;
+      l = __builtin_fmaf(ml.y, w, l);
+    }
+    o *= alpha;
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      if (s0 + i * W + own >= splits) break;
+      const float wi = __shfl(w, i * W + own);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(wi < 0.f ? 0.f : part[i][e], wi, o[e]);
+    }
   }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
   if constexpr (W > 1) {
     lds_o[wave][lane] = o;
     __syncthreads();
@@ -539,7 +552,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
     for (int i = 1; i < W; ++i) o += lds_o[wave + i][lane];
   }
   const float inv = __any(seen) ? 1.f / l : 0.f;  // a row whose scores are all -infinity is seen: not a number, as in one piece
-  if (live && lane * 4 < a.dim) {
+  if (live && !done && lane * 4 < a.dim) {
     const int64_t pos = r / a.group, head = hk * a.group + r % a.group;
     *reinterpret_cast<u32x2*>(a.out + b * a.o_b + pos * a.o_l + head * a.o_h + lane * 4) =
         u32x2{pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv)};

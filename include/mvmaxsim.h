@@ -475,7 +475,7 @@ MV_API int mv_enc_gated_act_bf16(int device, const void* d_gate, int64_t gate_ro
  *                  (x, y) -> scale * (x cos - y sin, y cos + x sin), x and y = elements (j, j + pairs), or (2 j, 2 j + 1) with adjacent != 0;
  *                  elements from 2 * pairs on are copied.  Angle of pair j = positions[axis[j]] * inv_freq[j] in 64 bits, or cos / sin tables
  *                  [batch][rows][pairs] by their strides (then positions must be NULL).  axis[j] must be an axis of positions.  Outputs may be the inputs
- *                  themselves (same pointer, same strides).  dtype MV_F32, MV_BF16 or MV_F16; 16-byte vectors where pairs and strides allow. */
+ *                  themselves (same pointer, same strides).  dtype MV_F32, MV_BF16 or MV_F16; pointers aligned to their elements, any strides. */
 typedef struct mv_rotary {
   const void *q, *k;
   void *q_out, *k_out;

@@ -153,25 +153,27 @@ class RotaryTable:
         return cls([theta ** (-j / share) for j in range(share)] * axes, [a for a in range(axes) for _ in range(share)], head_dim=head_dim, **kwargs)
 
 
-def _rotary_operands(torch, what, q, k, in_place):
-    """-> (q, k, their outputs as [batch, rows, heads, dim] or None, outputs as the caller shaped them)"""
-    if q is None and k is None:
+def _rotary_operands(what, q, k, in_place):
+    """-> (q, k as [batch, rows, heads, dim] or None, their outputs, the outputs as the caller shaped them, the first of q and k)"""
+    torch = _torch()
+    x = x_out = q_out = y = y_out = k_out = None
+    if q is not None:
+        x, x_out, q_out = _rotary_operand(torch, what, "q", q, in_place)
+    if k is not None:
+        y, y_out, k_out = _rotary_operand(torch, what, "k", k, in_place)
+        if x is not None:
+            a, b = x.shape, y.shape
+            if x.dtype is not y.dtype or a[0] != b[0] or a[1] != b[1] or a[3] != b[3]:
+                raise ValueError(f"{what}: q and k differ in type, batch, rows or head width ({tuple(a)} {x.dtype}, {tuple(b)} {y.dtype})")
+            if in_place and _share_memory(x, y):
+                raise ValueError(f"{what}: q and k cannot be turned in place, they share memory")
+    elif x is None:
         raise ValueError(f"{what}: neither q nor k")
-    x, xo, x_shaped = _rotary_operand(torch, what, "q", q, in_place)
-    y, yo, y_shaped = _rotary_operand(torch, what, "k", k, in_place)
-    if x is not None and y is not None:
-        a, b = x.shape, y.shape
-        if x.dtype is not y.dtype or a[0] != b[0] or a[1] != b[1] or a[3] != b[3]:
-            raise ValueError(f"{what}: q and k differ in type, batch, rows or head width ({tuple(a)} {x.dtype}, {tuple(b)} {y.dtype})")
-        if in_place and _share_memory(x, y):
-            raise ValueError(f"{what}: q and k cannot be turned in place, they share memory")
-    return x, y, xo, yo, (x_shaped, y_shaped)
+    return x, y, x_out, y_out, (q_out, k_out), y if x is None else x
 
 
 def _rotary_operand(torch, what, name, t, in_place):
-    if t is None:
-        return None, None, None
-    x = _heads4(t, what, name)
+    x = t if t.dim() == 4 else _heads4(t, what, name)
     if x.stride(3) != 1 and x.shape[3] > 1 and x.numel():
         raise ValueError(f"{what}: the elements of a head of {name} must lie next to each other")
     if not in_place:
@@ -186,27 +188,32 @@ _NO_STRIDES = (0, 0, 0)
 
 
 def _launch_rotary(torch, what, q, k, qo, ko, index, code, positions, pos_strides, freq, axis, cos, sin, table_strides, scale, wide_positions, adjacent, pairs):
-    batch, rows, heads, dim = q.shape if q is not None else k.shape
-    if q is None:
-        heads, at_q, at_qo, st_q, st_qo = 0, 0, 0, _NO_STRIDES, _NO_STRIDES
-    else:
-        at_q, at_qo, st_q, st_qo = q.data_ptr(), qo.data_ptr(), q.stride()[:3], qo.stride()[:3]
-    if k is None:
-        kv_heads, at_k, at_ko, st_k, st_ko = 0, 0, 0, _NO_STRIDES, _NO_STRIDES
-    else:
-        kv_heads, at_k, at_ko, st_k, st_ko = k.shape[2], k.data_ptr(), ko.data_ptr(), k.stride()[:3], ko.stride()[:3]
-    packed = _PACK_ROTARY.pack(at_q, at_k, at_qo, at_ko, *st_q, *st_k, *st_qo, *st_ko, positions, *pos_strides, freq, axis, cos, sin, *table_strides, scale, code,
-                               wide_positions, adjacent, batch, rows, heads, kv_heads, dim, pairs)
+    heads = kv_heads = at_q = at_k = at_qo = at_ko = q0 = q1 = q2 = k0 = k1 = k2 = qo0 = qo1 = qo2 = ko0 = ko1 = ko2 = 0
+    if q is not None:
+        batch, rows, heads, dim = q.shape
+        at_q, (q0, q1, q2, _) = q.data_ptr(), q.stride()
+        at_qo, (qo0, qo1, qo2, _) = (at_q, (q0, q1, q2, 1)) if qo is q else (qo.data_ptr(), qo.stride())
+    if k is not None:
+        batch, rows, kv_heads, dim = k.shape
+        at_k, (k0, k1, k2, _) = k.data_ptr(), k.stride()
+        at_ko, (ko0, ko1, ko2, _) = (at_k, (k0, k1, k2, 1)) if ko is k else (ko.data_ptr(), ko.stride())
+    p0, p1, p2 = pos_strides
+    t0, t1, t2 = table_strides
+    packed = _PACK_ROTARY.pack(at_q, at_k, at_qo, at_ko, q0, q1, q2, k0, k1, k2, qo0, qo1, qo2, ko0, ko1, ko2, positions, p0, p1, p2, freq, axis, cos, sin, t0, t1, t2, scale,
+                               code, wide_positions, adjacent, batch, rows, heads, kv_heads, dim, pairs)
     _lib.check(_lib.lib().mv_enc_rotary(index, packed, _stream(torch, index)))
 
 
 def _extent(x) -> Tuple[int, int]:
-    n = x.element_size() * (1 + sum((s - 1) * st for s, st in zip(x.shape, x.stride())))
-    return x.data_ptr(), x.data_ptr() + n
+    at = x.data_ptr()
+    n = x.numel() if x.is_contiguous() else 1 + sum((s - 1) * st for s, st in zip(x.shape, x.stride()))
+    return at, at + n * x.element_size()
 
 
 def _overlaps(x) -> bool:
     """Whether two elements of x can share memory: sorted by stride, every dimension must step past all that lies below it."""
+    if x.is_contiguous():
+        return False
     reach = 0
     for st, n in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
         if st <= reach:
@@ -243,8 +250,7 @@ def rotary(q: Any, k: Any, positions: Any, table: RotaryTable, *, in_place: bool
     what = "rotary"
     if not isinstance(table, RotaryTable):
         raise ValueError(f"{what}: table must be a RotaryTable")
-    x, y, xo, yo, shaped = _rotary_operands(torch, what, q, k, in_place)
-    first = x if x is not None else y
+    x, y, xo, yo, shaped, first = _rotary_operands(what, q, k, in_place)
     code = _dtype_code(torch, first.dtype, what, fp32=True)
     batch, rows, _, dim = first.shape
     if dim != table.head_dim:
@@ -255,16 +261,17 @@ def rotary(q: Any, k: Any, positions: Any, table: RotaryTable, *, in_place: bool
     if n == 3:
         pos = positions
     elif n == 2:  # [axes, rows] of packed rows where q has no batch, [batch, rows] of one axis where it has
-        pos = positions[:, None] if (q if q is not None else k).dim() == 3 else positions[None]
+        pos = positions[:, None] if (k if q is None else q).dim() == 3 else positions[None]
     else:
         pos = positions[None, None] if n == 1 else positions
-    if pos.dim() != 3 or pos.shape[1] not in (1, batch) or pos.shape[2] != rows:
+    p_shape = pos.shape
+    if len(p_shape) != 3 or p_shape[1] not in (1, batch) or p_shape[2] != rows:
         raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit {batch} x {rows} rows")
-    if pos.shape[0] < table.axes:
-        raise ValueError(f"{what}: positions have {pos.shape[0]} axes, the table needs {table.axes}")
+    if p_shape[0] < table.axes:
+        raise ValueError(f"{what}: positions have {p_shape[0]} axes, the table needs {table.axes}")
     index = _device_index(torch, what, first, pos, table.inv_freq, first if y is None else y)
     st = pos.stride()
-    _launch_rotary(torch, what, x, y, xo, yo, index, code, pos.data_ptr(), (st[0], st[1] if pos.shape[1] == batch else 0, st[2]), table.inv_freq.data_ptr(),
+    _launch_rotary(torch, what, x, y, xo, yo, index, code, pos.data_ptr(), (st[0], st[1] if p_shape[1] == batch else 0, st[2]), table.inv_freq.data_ptr(),
                    table.axis.data_ptr(), 0, 0, _NO_STRIDES, table.scale, int(pos.dtype is torch.int64), int(table.pairing == "adjacent"), table.pairs)
     return shaped
 
@@ -276,8 +283,7 @@ def rotary_tables(q: Any, k: Any, cos: Any, sin: Any, *, pairing: str = "halves"
     what = "rotary_tables"
     if pairing not in _PAIRINGS:
         raise ValueError(f"{what}: pairing {pairing!r} (one of {_PAIRINGS})")
-    x, y, xo, yo, shaped = _rotary_operands(torch, what, q, k, in_place)
-    first = x if x is not None else y
+    x, y, xo, yo, shaped, first = _rotary_operands(what, q, k, in_place)
     code = _dtype_code(torch, first.dtype, what, fp32=True)
     batch, rows, _, dim = first.shape
     if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:

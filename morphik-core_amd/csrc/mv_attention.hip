@@ -65,7 +65,8 @@ struct AttnArgs {
   int32_t rows, keys, kv_heads, group, dim, tiles, block_rows, causal;  // tiles: blocks of block_rows over rows * group
   int32_t full, splits;  // blocks [0, full) take a tile each; the tiles behind them are cut into `splits` runs of keys, one block each
   float* partial;        // of those: [tile - full][split][rows of a tile] x (dim sums, maximum, sum of weights, 2 unused)
-  float qk;    // scale * log2(e); with a cap: scale / cap * 2 log2(e)
+  float qk;    // scale * log2(e)
+  float turn;  // with a cap: scale / cap * 2 log2(e), so that the score is cap * tanh(s turn ln(2) / 2)
   float cap;   // cap * log2(e), 0 = none
 };
 
@@ -88,21 +89,45 @@ __device__ __forceinline__ float unpack(uint16_t h) {
   else return (float)__builtin_bit_cast(_Float16, h);
 }
 
-// log2 of the weight's numerator from the raw product q.k (see AttnArgs::qk)
-template <bool CAP>
-__device__ __forceinline__ float score(float s, float qk, float cap) {
-  if constexpr (CAP) {  // cap * tanh(x) = cap - 2 cap / (1 + e^2x): 2e-7 of the cap off at worst, far below the weights' rounding
-    const float e = __builtin_amdgcn_exp2f(s * qk);
-    return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);
-  } else {
-    return s * qk;
+// Capped scores, in log2: cap * tanh(x) of the raw product s = q.k, x = s scale / cap.
+//  - From the exponential, cap (1 - 2 / (1 + e^2x)): within 2^-22 of the CAP, which is no measure of a score that is small beside it.  For caps up to
+//    kNarrowCap that is 2^-15 of a weight at most (of the caps of 20 ... 50 that models use 2^-17), a sixteenth of the half step it is rounded by.
+//  - As x times a polynomial in x^2 for |x| < 1/2 (least largest relative error: 2^-26), so within 2^-22 of the score itself: far below the cap it is the
+//    uncapped score.  Wider caps take it, and the exponential where a wave holds a score that is further out.
+// us without a cap, with a narrow one, with a wide one: 2 x 4096 rows of 16 heads of 128 253, 314, 344; of 64 147, 222, 236; 4 x 2048 rows of 8 heads of 256
+// 130, 150, 172; 8464 rows of 16 heads of 80 456, 577, 668.  Tried for the wide ones: both forms and a select for every score (432 and 344 at 128 and 64
+// columns), one of two loops by the tile's largest score (31 and 41 spilled registers at 64 and 256).
+enum Cap { kNoCap, kNarrow, kWide };
+constexpr float kNarrowCap = 100.f;
+constexpr float kNear = 1.4426950408889634f;        // |s turn| of |x| = 1/2
+constexpr float kHalfLn2Sq = 0.12011325347955035f;  // (ln(2) / 2)^2: x^2 = (s turn)^2 of these
+__device__ __forceinline__ float cap_far(float s, float turn, float cap) {
+  return cap * __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * turn)), 1.f);  // twice the cap may be more than 32 bits hold
+}
+__device__ __forceinline__ float cap_near(float s, float qk, float turn) {
+  constexpr float k1 = -0.333331436f * kHalfLn2Sq, k2 = 0.13325879f * kHalfLn2Sq * kHalfLn2Sq, k3 = -0.0530455038f * kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq,
+                  k4 = 0.0172415134f * kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq;
+  const float y = s * turn, z = y * y;
+  return s * qk * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(k4, z, k3), z, k2), z, k1), z, 1.f);
+}
+
+// log2 of the weight's numerator from the raw product q.k
+template <int CAP>
+__device__ __forceinline__ float score(const AttnArgs& a, float s) {
+  if constexpr (CAP == kNoCap) return s * a.qk;
+  else if constexpr (CAP == kNarrow) return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.turn)), a.cap);
+  else {
+    const float near = cap_near(s, a.qk, a.turn);
+    const bool is_far = !(fabsf(s) * a.turn < kNear);
+    if (__builtin_expect(__any(is_far), 0) && is_far) return cap_far(s, a.turn, a.cap);
+    return near;
   }
 }
 
 // The rows of a wave once more, one key at a time with a select per key, for rows whose result is not finite: a matrix product with the
 // weight 0 of a masked key would carry that key's NaN or infinity into the row.  Rare by nature (only where masked places hold such values, or
 // where the row's own operands do), so it is simple rather than fast.
-template <bool BF16, bool CAP>
+template <bool BF16, int CAP>
 __device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int lo, int hi, uint16_t* out, float* partial) {
   const int lane = threadIdx.x & 63;
   float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -116,7 +141,7 @@ __device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* 
       if (c * 64 + lane < a.dim) s = __builtin_fmaf(qv[c], unpack<BF16>(k[(int64_t)j * a.k_l + c * 64 + lane]), s);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-    const float t = score<CAP>(s, a.qk, a.cap);
+    const float t = score<CAP>(a, s);
     const float m2 = t > m ? t : m;
     const float alpha = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m - m2);
     const float p = m2 == -INFINITY ? (t != t ? t : 0.f) : __builtin_amdgcn_exp2f(t - m2);
@@ -184,7 +209,7 @@ __device__ __forceinline__ float first_lane(float x) { return __int_as_float(uni
 // K/V head 133 us (1.03), 8464 rows of 16 heads of 80 444 us (0.83; the 16-column and 32-column steps round 80 up to 80 and 96).  Tried and not kept: two
 // groups of waves half a tile apart (289 us at 128), the weights of 32 keys beside the products of the next 32 (292), 64 rows a wave
 // (289, and 209 at 256), wave priorities (no change).
-template <bool BF16, int KC, bool CAP, int kWaves>
+template <bool BF16, int KC, int CAP, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(KC), waves_per_simd(KC)))) void attention_kernel(
     const AttnArgs a) {
   constexpr int kBlockRows = kWaves * kWaveRows;
@@ -333,7 +358,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
 
   f32x16 o[DT] = {};
   float m = -INFINITY, l = 0.f;
-  const float qk = CAP ? 1.f : a.qk;  // capped scores are logarithms already
+  const float qk = CAP == kNoCap ? a.qk : 1.f;  // capped scores are logarithms already
   if (k_lo < k_hi) fetch(k_lo, 0);
 
   int buf = 0;
@@ -364,11 +389,11 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
 
     const bool cut = k0 < in_lo || k0 + BK > in_hi;  // some row does not see some key of the tile
     s16x8 p[BK / 16];
-    if constexpr (CAP) {
+    if constexpr (CAP != kNoCap) {
 #pragma unroll
       for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[t][e] = score<true>(s[t][e], a.qk, a.cap);
+        for (int e = 0; e < 16; ++e) s[t][e] = score<CAP>(a, s[t][e]);
     }
     if (cut) {
       const int2 row = lds_rows[wave * kWaveRows + (lane & 31)];
@@ -624,7 +649,7 @@ int cu_count(int device) {
   return n;
 }
 
-template <bool BF16, int KC, bool CAP>
+template <bool BF16, int KC, int CAP>
 void launch_attention(const AttnArgs& a, int64_t blocks, hipStream_t s) {
   constexpr int kMany = block_waves(KC);
   if constexpr (kMany == 8) {
@@ -636,7 +661,7 @@ void launch_attention(const AttnArgs& a, int64_t blocks, hipStream_t s) {
   hipLaunchKernelGGL((attention_kernel<BF16, KC, CAP, kMany>), dim3((unsigned)blocks), dim3(kMany * 64), 0, s, a);
 }
 
-template <bool BF16, bool CAP>
+template <bool BF16, int CAP>
 void dispatch_dim(const AttnArgs& a, int64_t blocks, hipStream_t s) {
   switch (built_kc(a.dim)) {
     case 2: return launch_attention<BF16, 2, CAP>(a, blocks, s);
@@ -647,6 +672,13 @@ void dispatch_dim(const AttnArgs& a, int64_t blocks, hipStream_t s) {
     case 12: return launch_attention<BF16, 12, CAP>(a, blocks, s);
     default: return launch_attention<BF16, 16, CAP>(a, blocks, s);
   }
+}
+
+template <bool BF16>
+void dispatch_cap(const AttnArgs& a, float softcap, int64_t blocks, hipStream_t s) {
+  if (softcap == 0.f) dispatch_dim<BF16, kNoCap>(a, blocks, s);
+  else if (softcap <= kNarrowCap) dispatch_dim<BF16, kNarrow>(a, blocks, s);
+  else dispatch_dim<BF16, kWide>(a, blocks, s);
 }
 
 // ---------------------------------------------------------------- key ranges
@@ -736,13 +768,12 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   a.v_b = p->v_batch, a.v_l = v_row, a.v_h = p->v_head;
   a.o_h = p->dim, a.o_l = (int64_t)p->heads * p->dim, a.o_b = a.o_l * p->rows;
   a.rows = p->rows, a.keys = p->keys, a.kv_heads = p->kv_heads, a.group = p->heads / p->kv_heads, a.dim = p->dim, a.causal = p->causal && !p->ranges;
+  a.qk = p->scale * kLog2e;
   if (p->softcap > 0.f) {
-    a.qk = (float)((double)p->scale / p->softcap * 2.0 * 1.4426950408889634);
+    a.turn = (float)((double)p->scale / p->softcap * 2.0 * 1.4426950408889634);
     a.cap = p->softcap * kLog2e;
-  } else {
-    a.qk = p->scale * kLog2e;
   }
-  if (!(a.qk > 0.f) || !std::isfinite(a.qk) || !std::isfinite(a.cap)) {
+  if (!(a.qk > 0.f) || !std::isfinite(a.qk) || !std::isfinite(a.cap) || (p->softcap > 0.f && (!(a.turn > 0.f) || !std::isfinite(a.turn)))) {
     set_error("mv_enc_attention: scale or scale / softcap leaves 32 bits");
     return MV_ERR_INVALID;
   }
@@ -767,11 +798,9 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
     const int64_t words = (int64_t)p->batch * a.o_b / 2;
     hipLaunchKernelGGL(zero_rows_kernel, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4096)), dim3(256), 0, s, reinterpret_cast<uint32_t*>(a.out), words);
   } else if (p->dtype == MV_BF16) {
-    if (p->softcap > 0.f) dispatch_dim<true, true>(a, blocks, s);
-    else dispatch_dim<true, false>(a, blocks, s);
+    dispatch_cap<true>(a, p->softcap, blocks, s);
   } else {
-    if (p->softcap > 0.f) dispatch_dim<false, true>(a, blocks, s);
-    else dispatch_dim<false, false>(a, blocks, s);
+    dispatch_cap<false>(a, p->softcap, blocks, s);
   }
   MV_HIP(hipGetLastError());
   if (p->keys > 0 && pl.splits > 1) {

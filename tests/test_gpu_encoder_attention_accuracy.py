@@ -1,0 +1,64 @@
+"""Attention against its definition in 64 bits where its own arithmetic is the question: caps of every size.
+
+Tolerance per element, in terms of the row: p_j its weights, a = sum_j p_j |v_j|, e the largest sum_d |q_d k_d| * scale, n its keys, u half a step of the type
+(bf16 2^-8, fp16 2^-11).
+  result                      u |o|  (fp16 below 2^-14: 2^-25)
+  weights as operands         u a  (bf16 has the exponents of fp32)
+  scores, off by d each       2 d a: the numerators are off by at most d relative, and so is their sum
+    the dot product           d = (dim + 16) 2^-23 e
+    the cap                   d = 2^-20 |s| (a relative error of the capped score) or, up to caps of 100, 2^-21 cap at most: 100 * 2^-21 = 2^-14.3
+  sums and exponentials       (n + 64) 2^-23 a"""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_encoder_attention import DT, ea, gen, make  # noqa: F401  (ea: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def oracle(q, k, v, lo=None, hi=None, scale=None, softcap=0.0):
+    """-> (result, tolerance); one range of keys for all rows."""
+    batch, rows, heads, dim = q.shape
+    kv = k.shape[2]
+    k, v = k[:, lo:hi], v[:, lo:hi]
+    scale = dim**-0.5 if scale is None else scale
+    u = torch.finfo(q.dtype).eps / 2
+    out = torch.zeros(batch, rows, heads, dim, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    for b in range(batch):
+        for h in range(heads):
+            qq, kk, vv = q[b, :, h].double(), k[b, :, h // (heads // kv)].double(), v[b, :, h // (heads // kv)].double()
+            s = (qq @ kk.t().contiguous()) * scale
+            d = (dim + 16) * 2.0**-23 * ((qq.abs() @ kk.abs().t().contiguous()) * scale).amax(-1, keepdim=True)
+            if softcap:
+                s = softcap * torch.tanh(s / softcap)
+                d = d + torch.clamp(2.0**-20 * s.abs().amax(-1, keepdim=True), min=2.0**-21 * softcap if softcap <= 100 else 0.0)
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            p = p / p.sum(-1, keepdim=True)
+            o, a = p @ vv, p @ vv.abs()
+            out[b, :, h] = o
+            tol[b, :, h] = u * o.abs() + u * a + (2 * d + (vv.shape[0] + 64) * 2.0**-23) * a + (2.0**-25 if q.dtype == torch.float16 else 0.0)
+    return out, tol
+
+
+def check(got, want, tol, what):
+    assert got.shape == want.shape and bool(torch.isfinite(got).all()), what
+    off = (got.double() - want).abs()
+    assert bool((off <= tol).all()), f"{what}: {float(off.max()):.3e} off, {float((off - tol).max()):.3e} more than allowed"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cap", [0.5, 5.0, 30.0, 50.0, 100.0, 101.0, 1e3, 1e4, 1e6, 1e9, 1e20, 1e30, 2e38])
+def test_caps_of_every_size(ea, dtype, cap):  # noqa: F811
+    """A cap far above the scores leaves them as they are, whatever its size; scores around and above it are bent."""
+    g = gen(40)
+    for dim, rows, keys, heads, kv, spread in ((64, 33, 1000, 2, 1, 2.0), (128, 3, 700, 8, 2, 1.0), (256, 20, 90, 4, 2, 2.0), (72, 40, 200, 2, 2, 2.0), (32, 2, 4000, 2, 1, 3.0)):
+        q = make(g, 1, rows, heads, dim, DT[dtype], "split", spread)
+        k, v = make(g, 1, keys, kv, dim, DT[dtype], "split"), make(g, 1, keys, kv, dim, DT[dtype], "split")
+        check(ea.attention(q, k, v, softcap=cap), *oracle(q, k, v, softcap=cap), what=(dim, "scores of a few"))
+        if cap <= 1e4:  # scores a few times 0.05 times the factor: from far below to far above half the cap
+            for factor in (20.0, cap):
+                args = dict(softcap=cap, scale=factor / dim**0.5)
+                check(ea.attention(q * 0.05, k, v, **args), *oracle(q * 0.05, k, v, **args), what=(dim, factor))

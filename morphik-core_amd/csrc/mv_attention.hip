@@ -50,7 +50,11 @@ constexpr int kFewWaves = 2;  // of a block of a short call: see few_waves()
 // The widths that are built: a head takes the next wider one
 constexpr int built_kc(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : dim <= 128 ? 8 : dim <= 192 ? 12 : 16; }
 constexpr int kMatrix = 0x008, kDsRead = 0x100;  // classes of __builtin_amdgcn_sched_group_barrier
-constexpr float kRescale = 8.f;                // running maxima move only when a score passes them by 2^8: the weights stay <= 256
+// Running maxima m move only when a score passes them by 2^rescale, and weights are 2^(score - m + lift): bf16 has the exponents of 32 bits, but in fp16 a
+// weight below 2^-14 loses digits and one below 2^-25 is nothing, which thousands of weak keys beside a strong one miss (8463 keys 17.5 below it in e's
+// logarithm: 2e-4 of their values, gone).  So fp16 weights fill the type up to 2^15, and what is lost lies below 2^-36 of the row's sum a key.
+constexpr float rescale(bool bf16) { return bf16 ? 8.f : 4.f; }
+constexpr float lift(bool bf16) { return bf16 ? 0.f : 11.f; }
 
 // In place of a run's sum of weights: the row is not in pieces and done, the row sees nothing of the run
 constexpr float kDone = -1.f, kUnseen = -2.f;
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
     top = fmaxf(top, __shfl_xor(top, 32)) * qk;
-    if (__any(top > m + kRescale)) {
+    if (__any(top > m + rescale(BF16))) {
       const float m2 = fmaxf(m, top);
       const float alpha = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m2);
       m = m2;
@@ -421,8 +425,8 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    // weights, rounded to the operands' type for the matrix instruction (half a step of it, below the output's own rounding)
+    const float base = m == -INFINITY ? 0.f : m - lift(BF16);
+    // weights, rounded to the operands' type for the matrix instruction (half a step of it, like the result's own rounding)
 #pragma unroll
     for (int t = 0; t < BK / 32; ++t)
 #pragma unroll
@@ -488,7 +492,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
           *reinterpret_cast<u32x2*>(orow + d * 32 + e * 8 + half * 4) = nothing ? u32x2{0, 0} : w;
         }
   } else if (live_e) {
-    if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, kUnseen) : make_float2(m, l);
+    if (half == 0) *reinterpret_cast<float2*>(prow + a.dim) = nothing ? make_float2(-INFINITY, kUnseen) : make_float2(m - lift(BF16), l);
     if (!nothing) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)

@@ -1,9 +1,10 @@
-"""Attention against its definition in 64 bits where its own arithmetic is the question: caps of every size.
+"""Attention against its definition in 64 bits where its own arithmetic is the question: caps of every size, and fp16 weights
+far below a row's largest.
 
 Tolerance per element, in terms of the row: p_j its weights, a = sum_j p_j |v_j|, e the largest sum_d |q_d k_d| * scale, n its keys, u half a step of the type
 (bf16 2^-8, fp16 2^-11).
   result                      u |o|  (fp16 below 2^-14: 2^-25)
-  weights as operands         u a  (bf16 has the exponents of fp32)
+  weights as operands         u a  (bf16 has the exponents of fp32; of an fp16 weight at most 2^-36 of the row's sum is lost: 2^-36 sum_j |v_j|)
   scores, off by d each       2 d a: the numerators are off by at most d relative, and so is their sum
     the dot product           d = (dim + 16) 2^-23 e
     the cap                   d = 2^-20 |s| (a relative error of the capped score) or, up to caps of 100, 2^-21 cap at most: 100 * 2^-21 = 2^-14.3
@@ -39,7 +40,7 @@ def oracle(q, k, v, lo=None, hi=None, scale=None, softcap=0.0):
             p = p / p.sum(-1, keepdim=True)
             o, a = p @ vv, p @ vv.abs()
             out[b, :, h] = o
-            tol[b, :, h] = u * o.abs() + u * a + (2 * d + (vv.shape[0] + 64) * 2.0**-23) * a + (2.0**-25 if q.dtype == torch.float16 else 0.0)
+            tol[b, :, h] = u * o.abs() + u * a + (2 * d + (vv.shape[0] + 64) * 2.0**-23) * a + ((2.0**-25 + 2.0**-36 * vv.abs().sum(0)) if q.dtype == torch.float16 else 0.0)
     return out, tol
 
 
@@ -62,3 +63,22 @@ def test_caps_of_every_size(ea, dtype, cap):  # noqa: F811
             for factor in (20.0, cap):
                 args = dict(softcap=cap, scale=factor / dim**0.5)
                 check(ea.attention(q * 0.05, k, v, **args), *oracle(q * 0.05, k, v, **args), what=(dim, factor))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,keys", [(1, 300), (40, 8464), (300, 8464), (1, 20001), (2, 131072)])
+def test_thousands_of_weak_keys_beside_a_strong_one(ea, dtype, rows, keys):  # noqa: F811
+    """One key (first, in the middle or last) takes nearly all of the softmax and holds zeros, the others, 5 ... 22 below it, hold ones and twos: the result is
+    their share, in one piece and cut along the keys."""
+    dim = 64
+    for at in (0, keys // 2, keys - 1):
+        for gap in (5.0, 12.0, 17.0, 17.5, 18.0, 20.0, 22.0):
+            q = torch.zeros(1, rows, 2, dim, device="cuda")
+            k = torch.zeros(1, keys, 1, dim, device="cuda")
+            v = torch.ones(1, keys, 1, dim, device="cuda")
+            q[..., 0], q[:, :, 1, 1] = 8.0, 1.0
+            k[:, at, :, 0] = gap  # 8 * gap / sqrt(64)
+            k[:, :, 0, 1] = torch.linspace(-2, 2, keys, device="cuda")
+            v[..., 1::2], v[:, at] = 2.0, 0.0
+            q, k, v = (t.to(DT[dtype]) for t in (q, k, v))
+            check(ea.attention(q, k, v), *oracle(q, k, v), what=(at, gap))

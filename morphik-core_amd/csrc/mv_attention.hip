@@ -29,6 +29,7 @@ using f32x2 = __attribute__((ext_vector_type(2))) float;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using lds_u32x4 = __attribute__((address_space(3))) u32x4;
+using const_s16x8 = const __attribute__((address_space(4))) s16x8;
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -93,6 +94,8 @@ __device__ __forceinline__ float unpack(uint16_t h) {
   else return (float)__builtin_bit_cast(_Float16, h);
 }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Capped scores, in log2: cap * tanh(x) of the raw product s = q.k, x = s scale / cap.
 //  - From the exponential, cap (1 - 2 / (1 + e^2x)): within 2^-22 of the CAP, which is no measure of a score that is small beside it.  For caps up to
 //    kNarrowCap that is 2^-15 of a weight at most (of the caps of 20 ... 50 that models use 2^-17), a sixteenth of the half step it is rounded by.
@@ -128,40 +131,166 @@ __device__ __forceinline__ float score(const AttnArgs& a, float s) {
   }
 }
 
-// The rows of a wave once more, one key at a time with a select per key, for rows whose result is not finite: a matrix product with the
-// weight 0 of a masked key would carry that key's NaN or infinity into the row.  Rare by nature (only where masked places hold such values, or
-// where the row's own operands do), so it is simple rather than fast.
-template <bool BF16, int CAP>
-__device__ void exact_row(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int lo, int hi, uint16_t* out, float* partial) {
+// Which rows of a wave (a bit each) may owe a result that is not finite to something they do not see.  In the matrix products a value that is not finite
+// counts even under a zero: the values of a masked key of the tile under its weight, and in heads narrower than the kernel an infinite first chunk of K,
+// which stands in for the columns that q holds zeros for.  All other rows are right as they are, also those that are not a number by a score of their own.
+// One lane a key, over the tiles that this wave worked on; q, lo and hi are the lane's row and its range.
+template <bool BF16, int KC, int CAP>
+__device__ uint32_t spoiled_rows(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int k_lo, int k_hi, int w_lo, int w_hi, int in_lo, int in_hi, int lo, int hi) {
+  constexpr int BK = tile_keys(KC);
+  constexpr uint32_t kTop = BF16 ? 0x7f80 : 0x7c00;  // all bits of the exponent
   const int lane = threadIdx.x & 63;
-  float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool narrow = a.dim < KC * 16;
+  bool hit = false, lost = false;
+  for (int k0 = k_lo; k0 < k_hi; k0 += BK) {
+    const bool cut = k0 < in_lo || k0 + BK > in_hi;
+    if (k0 + BK <= w_lo || k0 >= w_hi || !(cut || narrow)) continue;
+    const bool mine = lane < BK && k0 + lane < k_hi;
+    bool odd = false, inf = false;
+    if (mine && cut) {
+      const uint16_t* row = v + (int64_t)(k0 + lane) * a.v_l;
+#pragma unroll 4
+      for (int c = 0; c < a.dim; c += 8) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(row + c);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) qv[c] = c * 64 + lane < a.dim ? unpack<BF16>(q[c * 64 + lane]) : 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    float s = 0.f;
+        for (int e = 0; e < 4; ++e) odd |= (w[e] & kTop) == kTop || (w[e] & kTop << 16) == kTop << 16;
+      }
+    }
+    if (mine && narrow) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(k + (int64_t)(k0 + lane) * a.k_l);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 64 + lane < a.dim) s = __builtin_fmaf(qv[c], unpack<BF16>(k[(int64_t)j * a.k_l + c * 64 + lane]), s);
+      for (int e = 0; e < 4; ++e) inf |= (w[e] & 0x7fff) == kTop || (w[e] >> 16 & 0x7fff) == kTop;
+    }
+    const uint64_t odds = __ballot(odd), infs = __ballot(inf);
+    const int from = min(max(lo - k0, 0), 64), to = min(max(hi - k0, 0), 64);
+    const uint64_t sees = from < to ? ~0ull >> (64 - (to - from)) << from : 0;
+    hit |= ((odds & ~sees) | (infs & sees)) != 0;
+    if (CAP != kNoCap) continue;  // a cap makes every infinite score finite
+    for (uint64_t left = infs; left; left &= left - 1) {
+      const int at = __builtin_ctzll(left);
+      const bool asks = sees >> at & 1 && !lost;
+      if (!__any(asks)) continue;
+      const uint16_t* row = k + (int64_t)(k0 + at) * a.k_l;
+      float s = 0.f;
+      if (asks) {
+#pragma unroll 2
+        for (int c = 0; c < a.dim; c += 8) {
+          const s16x8 qc = *reinterpret_cast<const s16x8*>(q + c), kc = *reinterpret_cast<const s16x8*>(row + c);
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-    const float t = score<CAP>(a, s);
-    const float m2 = t > m ? t : m;
-    const float alpha = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m - m2);
-    const float p = m2 == -INFINITY ? (t != t ? t : 0.f) : __builtin_amdgcn_exp2f(t - m2);
-    m = m2;
-    l = __builtin_fmaf(l, alpha, p);
+          for (int e = 0; e < 8; ++e) s = __builtin_fmaf(unpack<BF16>((uint16_t)qc[e]), unpack<BF16>((uint16_t)kc[e]), s);
+        }
+        lost = s != -INFINITY;
+      }
+    }
+  }
+  const uint64_t hits = __ballot(hit && !lost);
+  return (uint32_t)(hits | hits >> 32);
+}
+
+// Those rows once more, R of them at a time by a whole wave, with what a row does not see selected away: scores one key a lane, then the 64 keys'
+// values, four columns a lane.
+struct AgainRow {
+  const uint16_t* q;
+  uint16_t* out;
+  float* partial;
+  int lo, hi;
+};
+template <bool BF16, int CAP, int R>
+__device__ void exact_rows(const AttnArgs& a, const AgainRow (&rows)[R], int count, const uint16_t* k, const uint16_t* v) {
+  const int lane = threadIdx.x & 63, col = lane * 4;
+  f32x4 o[R];
+  float m[R], l[R];
+  int from = 0x7fffffff, to = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 64 + lane < a.dim) o[c] = __builtin_fmaf(o[c], alpha, p * unpack<BF16>(v[(int64_t)j * a.v_l + c * 64 + lane]));
+  for (int r = 0; r < R; ++r) {
+    o[r] = f32x4{}, m[r] = -INFINITY, l[r] = 0.f;
+    from = min(from, rows[r].lo), to = max(to, rows[r].hi);
+  }
+  for (int j0 = from; j0 < to; j0 += 64) {
+    const int n = min(to - j0, 64), j = j0 + lane;
+    const uint16_t* kr = k + (int64_t)(j0 + min(lane, n - 1)) * a.k_l;
+    float s[R] = {};
+#pragma unroll 2
+    for (int c = 0; c < a.dim; c += 8) {
+      const s16x8 kc = *reinterpret_cast<const s16x8*>(kr + c);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const s16x8 qc = *(const_s16x8*)(uintptr_t)(rows[r].q + c);  // the same for all lanes: a scalar load
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[r] = __builtin_fmaf(unpack<BF16>((uint16_t)qc[e]), unpack<BF16>((uint16_t)kc[e]), s[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool sees = j >= rows[r].lo && j < rows[r].hi;
+      const float t = score<CAP>(a, s[r]);
+      float m2 = sees ? fmaxf(m[r], t) : m[r];
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) m2 = fmaxf(m2, __shfl_xor(m2, x));
+      const float alpha = m2 == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - m2);
+      const float p = m2 == -INFINITY ? (t != t ? t : 0.f) : __builtin_amdgcn_exp2f(t - m2);
+      m[r] = m2;
+      l[r] = __builtin_fmaf(l[r], alpha, sees ? p : 0.f);
+      o[r] *= alpha;
+      s[r] = sees ? p : -1.f;  // not seen
+    }
+    const uint16_t* vr = v + (int64_t)j0 * a.v_l + (col < a.dim ? col : 0);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i, vr += a.v_l) {
+      const s16x4 vc = *reinterpret_cast<const s16x4*>(vr);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[r]), i));
+        if (w < 0.f) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][e] = __builtin_fmaf(w, unpack<BF16>((uint16_t)vc[e]), o[r][e]);
+      }
+    }
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (c * 64 + lane < a.dim) {
-      if (partial) partial[c * 64 + lane] = o[c];
-      else out[c * 64 + lane] = (uint16_t)pack2<BF16>(o[c] / l, 0.f);
+  for (int r = 0; r < R; ++r) {
+    if (r >= count) break;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l[r] += __shfl_xor(l[r], x);
+    if (col < a.dim) {
+      if (rows[r].partial) *reinterpret_cast<f32x4*>(rows[r].partial + col) = o[r];
+      else *reinterpret_cast<u32x2*>(rows[r].out + col) = u32x2{pack2<BF16>(o[r][0] / l[r], o[r][1] / l[r]), pack2<BF16>(o[r][2] / l[r], o[r][3] / l[r])};
     }
-  if (partial && lane == 0) *reinterpret_cast<float2*>(partial + a.dim) = make_float2(m, l);
+    if (rows[r].partial && lane == 0) *reinterpret_cast<float2*>(rows[r].partial + a.dim) = make_float2(m[r], l[r]);
+  }
+}
+
+using const_args = const __attribute__((address_space(4))) AttnArgs;
+
+// The end of a wave with rows (a bit each in `again`) whose result is not finite.  2048 rows of 8 heads of 128 in 46 us: 46 when every row sees an infinite
+// value, 106 when a causal mask hides it from the rows in front of it, 205 in pages beside it.  Not inlined, and with the kernel's arguments read anew:
+// inlined, its scalar registers crowd the loop's (4 x 2048 rows of heads of 256 136 -> 145 us).
+template <bool BF16, int KC, int CAP>
+__attribute__((noinline)) __device__ void mend_rows(const_args* args, uint32_t again_, int b_, int hk_, int pos, int head, int lo, int hi, int k_lo_, int k_hi_, int w_lo_, int w_hi_, int in_lo_,
+                                                    int in_hi_, float* partial_, bool cut_) {
+  const uint64_t at = (uint64_t)args;
+  const AttnArgs& a = *(const AttnArgs*)(const_args*)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at));
+  const int b = uniform(b_), hk = uniform(hk_);
+  const uint16_t *k = a.k + b * a.k_b + hk * a.k_h, *v = a.v + b * a.v_b + hk * a.v_h;
+  float* partial = uniform(cut_) ? partial_ : nullptr;
+  uint32_t again = uniform(again_);
+  again &= spoiled_rows<BF16, KC, CAP>(a, a.q + b * a.q_b + (int64_t)pos * a.q_l + head * a.q_h, k, v, uniform(k_lo_), uniform(k_hi_), uniform(w_lo_), uniform(w_hi_),
+                                       uniform(in_lo_), uniform(in_hi_), lo, hi);
+  while (again) {
+    constexpr int kAgain = 8;
+    AgainRow rows[kAgain];
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kAgain; ++i) {
+      const int src = again ? __builtin_ctz(again) : 0;
+      const int64_t pos2 = uniform(__shfl(pos, src)), head2 = uniform(__shfl(head, src));
+      rows[i] = {a.q + b * a.q_b + pos2 * a.q_l + head2 * a.q_h, a.out + b * a.o_b + pos2 * a.o_l + head2 * a.o_h, partial ? partial + src * (a.dim + 4) : nullptr,
+                 again ? uniform(__shfl(lo, src)) : 0x7fffffff, again ? uniform(__shfl(hi, src)) : 0};
+      count += again != 0;
+      again &= again - 1;
+    }
+    exact_rows<BF16, CAP, kAgain>(a, rows, count, k, v);
+  }
 }
 
 // Where a 16-byte chunk of a staged row lies: chunk c of row r at r * CH + (c ^ swizzle(r)).  LDS serves 256 bytes a cycle: 16 lanes of a K read
@@ -194,7 +323,6 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_
 }
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float first_lane(float x) { return __int_as_float(uniform(__float_as_int(x))); }
 
 // One block: 32 rows a wave against the keys that any of them sees, in tiles of BK keys staged through LDS.
@@ -502,15 +630,8 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
             *reinterpret_cast<f32x4*>(prow + d * 32 + e * 8 + half * 4) = f32x4{o[d][e * 4], o[d][e * 4 + 1], o[d][e * 4 + 2], o[d][e * 4 + 3]};
     }
   }
-  uint64_t again = __ballot(bad);
-  again = (again | again >> 32) & 0xffffffffu;
-  while (again) {
-    const int src = __builtin_ctzll(again);
-    again &= again - 1;
-    const int pos2 = __shfl(pos, src), head2 = __shfl(head, src), lo2 = __shfl(lo_s, src), hi2 = __shfl(hi_s, src);
-    exact_row<BF16, CAP>(a, a.q + b * a.q_b + (int64_t)pos2 * a.q_l + head2 * a.q_h, kb, vb, lo2, hi2, a.out + b * a.o_b + (int64_t)pos2 * a.o_l + head2 * a.o_h,
-                         partial ? partial + (wave * kWaveRows + src) * (a.dim + 4) : nullptr);
-  }
+  const uint64_t bads = __ballot(bad);
+  if (bads) mend_rows<BF16, KC, CAP>((const_args*)__builtin_amdgcn_kernarg_segment_ptr(), (uint32_t)(bads | bads >> 32), b, hk, pos, head, lo_s, hi_s, k_lo, k_hi, w_lo, w_hi, in_lo, in_hi, partial + wave * kWaveRows * (a.dim + 4), partial != nullptr);
 }
 
 // Joins the runs of keys of the cut tiles: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, join_runs of a wave at a time with the maximum moving as

@@ -1,5 +1,5 @@
-"""Attention against its definition in 64 bits where its own arithmetic is the question: caps of every size, and fp16 weights
-far below a row's largest.
+"""Attention against its definition in 64 bits where its own arithmetic is the question: caps of every size, fp16 weights
+far below a row's largest, operands that are not finite.
 
 Tolerance per element, in terms of the row: p_j its weights, a = sum_j p_j |v_j|, e the largest sum_d |q_d k_d| * scale, n its keys, u half a step of the type
 (bf16 2^-8, fp16 2^-11).
@@ -11,10 +11,13 @@ Tolerance per element, in terms of the row: p_j its weights, a = sum_j p_j |v_j|
   sums and exponentials       (n + 64) 2^-23 a"""
 import math
 
+import math
+
 import pytest
 import torch
 
 from tests.test_gpu_encoder_attention import DT, ea, gen, make  # noqa: F401  (ea: the fixture)
+from tests.test_gpu_encoder_attention import oracle as ranges_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +85,64 @@ def test_thousands_of_weak_keys_beside_a_strong_one(ea, dtype, rows, keys):  # n
             v[..., 1::2], v[:, at] = 2.0, 0.0
             q, k, v = (t.to(DT[dtype]) for t in (q, k, v))
             check(ea.attention(q, k, v), *oracle(q, k, v), what=(at, gap))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [40, 72, 80, 128, 256])
+@pytest.mark.parametrize("rows,keys", [(70, 200), (3, 2500), (600, 600)])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them_and_no_others(ea, dtype, dim, rows, keys):  # noqa: F811
+    """Infinite and NaN values at a few keys, rows with ranges of their own: where a row sees them, the columns that hold them are what the sum is (an infinity
+    of one sign, else NaN) and the other columns stay; rows that do not see them stay altogether.  The keys' scores are near each other, so that no weight
+    is rounded to 0."""
+    g = gen(dim + keys)
+    q, k, v = (make(g, 1, n, h, dim, DT[dtype], "heads", x) for n, h, x in ((rows, 4, 0.3), (keys, 2, 1.0), (keys, 2, 1.0)))
+    lo = torch.randint(0, keys, (1, rows), generator=g, device="cuda")
+    hi = torch.maximum(lo, torch.randint(0, keys + 1, (1, rows), generator=g, device="cuda"))
+    r = torch.stack([lo, hi], -1).to(torch.int32)
+    r[:, ::5] = torch.tensor([0, keys], dtype=torch.int32, device="cuda")
+    want, tol = ranges_oracle(q, k, v, r)
+    held = {keys // 3: (0, math.inf), keys // 3 + 1: (1, -math.inf), keys // 2: (dim - 1, math.nan), keys // 2 + 9: (0, -math.inf), keys - 2: (7, math.inf)}
+    v2, seen = v.clone(), {}
+    for at, (col, x) in held.items():
+        v2[:, at, :, col] = x
+        sees = (r[0, :, 0] <= at) & (at < r[0, :, 1])
+        seen.setdefault(col, []).append((x, sees))
+    got = ea.attention(q, k, v2, key_ranges=r)
+    for col, marks in seen.items():
+        total = sum(torch.where(s, x, 0.0) for x, s in marks)  # inf - inf and NaN come out as they do in the row's own sum
+        odd = ~torch.isfinite(total)
+        assert torch.equal(got[0, odd, :, col].float().nan_to_num(7.0, 8.0, 9.0), total[odd, None].expand(-1, 4).float().nan_to_num(7.0, 8.0, 9.0))
+        got[0, odd, :, col], want[0, odd, :, col] = 0, 0
+    check(got, want, tol, "the others")
+
+
+@pytest.mark.parametrize("dim", [72, 80, 128, 256])
+def test_a_value_that_is_not_finite_does_not_hold_up_the_call(ea, dim):  # noqa: F811
+    """A page whose activations overflowed takes up to a few times as long (measured: 1.0 ... 4.5 times, 17 where the heads are narrower than the kernel and K is
+    infinite in its first columns), not hundreds of times (161 ... 253 in the form that took every such row again key by key)."""
+    g = gen(dim)
+    rows = 2048
+    q, k, v = (make(g, 1, rows, h, dim, torch.float16, "split") for h in (8, 8, 8))
+    full = torch.full((1,), rows, dtype=torch.int32, device="cuda")
+    causal = ea.padded_ranges(torch.zeros_like(full), full, rows, prefix=0)
+    pages = ea.document_ranges(torch.tensor([0, 700, 1000, rows], dtype=torch.int32, device="cuda"), rows)
+
+    def us(q, k, v, r):
+        events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        for _ in range(2):
+            events[0].record()
+            out = ea.attention(q, k, v, key_ranges=r)
+            events[1].record()
+            events[1].synchronize()
+        return events[0].elapsed_time(events[1]) * 1e3, out
+
+    for name, r in (("all", None), ("causal", causal), ("pages", pages)):
+        clean = min(us(q, k, v, r)[0] for _ in range(3))
+        for what in ("q", "k", "v"):
+            for x in (math.inf, math.nan):
+                bad = [t.clone() for t in (q, k, v)]
+                bad["qkv".index(what)][:, 900, :, 5] = x
+                took, out = us(*bad, r)
+                print(f"{dim} {name} {what} {x}: {took / clean:.2f} of {clean:.0f} us")
+                assert not bool(torch.isfinite(out[:, 950]).all()) or what == "q"
+                assert took <= (12 if dim != 72 else 40) * clean + 100, (name, what, x, took, clean)

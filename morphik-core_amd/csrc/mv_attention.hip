@@ -61,6 +61,7 @@ constexpr float lift(bool bf16) { return bf16 ? 0.f : 11.f; }
 constexpr float kDone = -1.f, kUnseen = -2.f;
 
 constexpr int64_t kMaxRowStride = 1 << 23;    // elements: a tile's byte offsets stay below 2^31
+constexpr int64_t kMaxThreads = 0xffffffff;   // of a launch
 
 struct AttnArgs {
   const uint16_t *q, *k, *v;
@@ -905,7 +906,7 @@ int mv_enc_attention(int device, const mv_attn* p, void* stream) {
   const int64_t tall = (int64_t)p->rows * a.group;  // rows of one K/V head
   const Plan pl = plan(p->batch, p->rows, p->keys, p->heads, p->kv_heads, p->dim, cu_count(device));
   const int64_t blocks = pl.full + pl.cut * pl.splits;
-  if (tall > 0x7ffff000 || pl.blocks > 0x7fffffff || blocks > 0x7fffffff) {
+  if (tall > 0x7ffff000 || pl.blocks > 0x7fffffff || blocks * pl.waves * 64 > kMaxThreads) {
     set_error("mv_enc_attention: too many rows for one launch");
     return MV_ERR_INVALID;
   }
@@ -952,7 +953,7 @@ int mv_enc_padded_ranges(int device, const int32_t* d_starts, int64_t starts_str
   }
   const int64_t total = (int64_t)batch * rows;
   if (total == 0) return MV_OK;
-  if ((total + 255) / 256 > 0x7fffffff) {
+  if ((total + 255) / 256 * 256 > kMaxThreads) {
     set_error("mv_enc_padded_ranges: too many rows");
     return MV_ERR_INVALID;
   }

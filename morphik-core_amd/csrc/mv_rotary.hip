@@ -235,7 +235,7 @@ int mv_enc_rotary(int device, const mv_rotary* p, void* stream) {
   tokens = std::min<int64_t>(tokens, std::max<int64_t>(1, 32768 / std::max<int64_t>(8, (int64_t)p->pairs * 8)));
   a.tokens = (int32_t)std::min<int64_t>(tokens, total);
   const int64_t blocks = (total + a.tokens - 1) / a.tokens;
-  if (blocks > 0x7fffffff || (int64_t)a.tokens * (p->heads + p->kv_heads) * p->dim > 0x7fffffff) {
+  if (blocks * 256 > 0xffffffff /* threads of a launch */ || (int64_t)a.tokens * (p->heads + p->kv_heads) * p->dim > 0x7fffffff) {
     set_error("mv_enc_rotary: too many tokens or heads for one launch");
     return MV_ERR_INVALID;
   }

@@ -225,6 +225,16 @@ def test_the_c_entries_refuse_bad_structs_before_any_launch():
     assert L.mv_enc_document_ranges(0, None, 1, None, -1, 0, None, None) == 0
 
 
+def test_calls_of_more_threads_than_a_launch_holds_are_refused():
+    """2^32 threads and more: a refusal of the entry's own, not the launch's error."""
+    L = _lib.lib()
+    p = _lib.AttnC(q=16, k=16, v=16, out=16, dtype=_lib.MV_BF16, batch=65536, rows=1, keys=1, heads=128, kv_heads=128, dim=8, scale=1.0)
+    assert L.mv_enc_attention(0, C.byref(p), None) == -1 and "too many rows" in L.mv_last_error().decode()
+    r = _lib.RotaryC(q=16, k=16, q_out=16, k_out=16, dtype=_lib.MV_BF16, batch=2, rows=0x7FFFFFFF, heads=2, kv_heads=1, dim=16, pairs=8, positions=16, inv_freq=16, axis=16)
+    assert L.mv_enc_rotary(0, C.byref(r), None) == -1 and "too many tokens" in L.mv_last_error().decode()
+    assert L.mv_enc_padded_ranges(0, 16, 1, 16, 1, None, -1, 3, 0x7FFFFFFF, 0, 16, None) == -1 and "too many rows" in L.mv_last_error().decode()
+
+
 def test_scales_that_leave_32_bits_are_refused():
     q, k, v = qkv()
     with pytest.raises(ValueError, match="scale"):

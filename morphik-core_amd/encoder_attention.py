@@ -14,7 +14,7 @@ infinity included) does not reach the row.
 
 Everything is enqueued on torch's current stream of the tensors' device, allocates through torch only, keeps nothing between calls and may be
 captured into a graph.  These are inference operators, as the encoders run them: nothing here has a gradient, and tensors that would need one
-are refused.  There is no CPU path: tensors off the GPU are refused.
+(in either mode of autograd) are refused.  There is no CPU path: tensors off the GPU are refused.
 """
 from __future__ import annotations
 
@@ -69,11 +69,21 @@ def _device_index(torch, what: str, *tensors: Any) -> int:
     for t in tensors:
         if t.get_device() != index:
             raise ValueError(f"{what}: tensors on different devices ({tensors[0].device}, {t.device})")
+    _refuse_derivatives(torch, what, tensors)
+    return index
+
+
+def _refuse_derivatives(torch, what: str, tensors: Sequence[Any]) -> None:
+    """Neither mode of autograd follows these operators: a tensor that it would follow is refused, not dropped from the derivative."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
                 raise ValueError(f"{what}: has no gradient (run it under torch.inference_mode() or torch.no_grad())")
-    return index
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and torch._C._is_fwd_grad_enabled():  # inside a dual level only: asking costs 1 us a tensor
+        for t in tensors:
+            if forward.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what}: has no gradient (an operand carries a forward-mode tangent)")
 
 
 def _stream(torch, index: int) -> int:

@@ -146,3 +146,23 @@ def test_a_value_that_is_not_finite_does_not_hold_up_the_call(ea, dim):  # noqa:
                 print(f"{dim} {name} {what} {x}: {took / clean:.2f} of {clean:.0f} us")
                 assert not bool(torch.isfinite(out[:, 950]).all()) or what == "q"
                 assert took <= (12 if dim != 72 else 40) * clean + 100, (name, what, x, took, clean)
+
+
+def test_forward_mode_tangents_are_refused(ea):  # noqa: F811
+    from torch.autograd import forward_ad
+
+    g = gen(43)
+    q, k, v = (make(g, 1, 4, 2, 16, torch.bfloat16, "split") for _ in range(3))
+    table, pos = ea.RotaryTable.with_sections(16, [8]), torch.zeros(4, dtype=torch.int64, device="cuda")
+    cos = torch.ones(1, 4, 8, device="cuda")
+    with forward_ad.dual_level():
+        for bad in range(3):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == bad else t for i, t in enumerate((q, k, v))]
+            with pytest.raises(ValueError, match="tangent"):
+                ea.attention(*args)
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        with pytest.raises(ValueError, match="tangent"):
+            ea.rotary(q, dual, pos, table)
+        with pytest.raises(ValueError, match="tangent"):
+            ea.rotary_tables(q, k, cos, forward_ad.make_dual(cos, torch.ones_like(cos)))
+        assert ea.attention(q, k, v).shape == q.shape and ea.rotary(q, k, pos, table)[0].shape == q.shape

@@ -549,7 +549,10 @@ def _decoder_forward(self, *args, **kwargs):
     if mask is not None:
         out = attention(q, k, v, key_ranges=mask[:, 0], scale=self.scaling)
     else:
-        out = attention(q, k, v, causal=self.is_causal and rows > 1, scale=self.scaling)
+        causal = self.is_causal and rows > 1
+        if causal and k.shape[1] > rows:  # no mask over a longer cache: a prompt in front of its unfilled places
+            k, v = k[:, :rows], v[:, :rows]
+        out = attention(q, k, v, causal=causal, scale=self.scaling)
     return self.o_proj(out.flatten(2)), None
 
 

@@ -1,0 +1,50 @@
+"""Patched encoder modules beside the modules they replace: calls in which the two must not differ in what they compute."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ea():
+    from morphik_core_amd import encoder_attention
+
+    assert torch.cuda.is_available()
+    yield encoder_attention
+    torch.cuda.empty_cache()
+
+
+def gemma(**config):
+    """A small random Gemma decoder in bf16 on the GPU."""
+    from transformers import GemmaConfig, GemmaModel
+
+    cfg = GemmaConfig(**{**dict(hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=32, vocab_size=100), **config})
+    torch.manual_seed(3)
+    return GemmaModel(cfg).to(torch.bfloat16).cuda().eval()
+
+
+def ids(batch=2, rows=9, seed=4):
+    return torch.randint(1, 100, (batch, rows), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def near(a, b):
+    """Hidden states of unit scale after two bf16 blocks: sums of roundings of 2^-8 each, far below what one wrong key does to a row."""
+    off = (a.float() - b.float()).norm(dim=-1) / b.float().norm(dim=-1)
+    return float(off.max()) < 0.05
+
+
+def test_a_prompt_in_front_of_an_empty_static_cache_sees_itself_only(ea):
+    """The cache hands back all of its places, the mask is left to `causal`: row i sees the keys up to i, not the unfilled ones behind them."""
+    from transformers import StaticCache
+
+    model, x = gemma(), ids()
+    with torch.inference_mode():
+        plain = model(input_ids=x).last_hidden_state
+        ea.patch_attention(model)
+        want = model(input_ids=x).last_hidden_state
+        cache = StaticCache(config=model.config, max_cache_len=40)
+        got = model(input_ids=x, past_key_values=cache, use_cache=True).last_hidden_state
+        assert torch.equal(got, want) and near(want, plain)
+        nxt = ids(rows=1, seed=5)  # and the token behind it, whose mask is one of key ranges
+        got = model(input_ids=nxt, past_key_values=cache, use_cache=True).last_hidden_state
+        assert near(got, model(input_ids=torch.cat([x, nxt], 1)).last_hidden_state[:, -1:])

@@ -481,12 +481,16 @@ def _kernel_takes(torch, *tensors) -> bool:
                for t in tensors)
 
 
+def _is_causal(module, asked: Optional[bool]) -> bool:
+    """Without a mask: what the forward asks for, else what the module says; one that says nothing is causal, as the framework's own function takes it."""
+    return bool(getattr(module, "is_causal", True) if asked is None else asked)
+
+
 def _interface_attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, softcap=None, is_causal=None, **kwargs):
     """transformers' attention function: query [batch, heads, rows, dim], key / value [batch, kv_heads, keys, dim] -> ([batch, rows, heads, dim], None)."""
     torch = _torch()
     ranges = attention_mask[:, 0] if attention_mask is not None and attention_mask.dtype == torch.int32 else None
-    causal = getattr(module, "is_causal", False) if is_causal is None else is_causal
-    causal = bool(causal) and attention_mask is None and query.shape[2] > 1
+    causal = attention_mask is None and query.shape[2] > 1 and _is_causal(module, is_causal)
     known = ranges is not None or attention_mask is None and not (causal and query.shape[2] != key.shape[2])
     extras = any(kwargs.get(name) is not None for name in ("s_aux", "position_bias"))  # sinks, added biases: not in the kernel
     if known and not dropout and not extras and _kernel_takes(torch, query, key, value):
@@ -549,7 +553,7 @@ def _decoder_forward(self, *args, **kwargs):
     if mask is not None:
         out = attention(q, k, v, key_ranges=mask[:, 0], scale=self.scaling)
     else:
-        causal = self.is_causal and rows > 1
+        causal = rows > 1 and _is_causal(self, kwargs.get("is_causal"))
         if causal and k.shape[1] > rows:  # no mask over a longer cache: a prompt in front of its unfilled places
             k, v = k[:, :rows], v[:, :rows]
         out = attention(q, k, v, causal=causal, scale=self.scaling)

@@ -48,3 +48,30 @@ def test_a_prompt_in_front_of_an_empty_static_cache_sees_itself_only(ea):
         nxt = ids(rows=1, seed=5)  # and the token behind it, whose mask is one of key ranges
         got = model(input_ids=nxt, past_key_values=cache, use_cache=True).last_hidden_state
         assert near(got, model(input_ids=torch.cat([x, nxt], 1)).last_hidden_state[:, -1:])
+
+
+def test_without_a_mask_the_forward_then_the_module_say_whether_rows_are_causal(ea):
+    """is_causal= of a forward reaches the blocks; a module that says nothing counts as causal, as for the framework's own function."""
+    from transformers import AttentionInterface
+
+    model, x = gemma(), ids()
+    with torch.inference_mode():
+        plain = [model(input_ids=x, **kw).last_hidden_state for kw in ({}, dict(is_causal=False), dict(is_causal=True))]
+        assert not near(plain[0], plain[1])
+        ea.patch_attention(model)
+        for want, kw in zip(plain, ({}, dict(is_causal=False), dict(is_causal=True))):
+            assert near(model(input_ids=x, **kw).last_hidden_state, want)
+
+    class Says(torch.nn.Module):
+        def __init__(self, **said):
+            super().__init__()
+            for name, value in said.items():
+                setattr(self, name, value)
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(1, 2, 7, 32, generator=g, device="cuda").to(torch.bfloat16) for _ in range(3))
+    with torch.inference_mode():
+        for module in (Says(), Says(is_causal=True), Says(is_causal=False)):
+            for asked in (None, True, False):
+                got = ea._interface_attention(module, q, k, v, is_causal=asked)[0]
+                assert near(got, AttentionInterface()["sdpa"](module, q, k, v, None, is_causal=asked)[0])

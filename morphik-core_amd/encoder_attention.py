@@ -537,12 +537,17 @@ def _rotary_forward(self, x, position_ids, *args, **kwargs):
     return out
 
 
+def _drops(module) -> bool:
+    """Training mode (under no_grad) with dropout of the attention's weights: not in the kernel."""
+    return bool(module.training and getattr(module, "attention_dropout", 0.0))
+
+
 def _decoder_forward(self, *args, **kwargs):
     """q, k, v -> rotation in place -> attention over key ranges -> output projection; what does not fit goes through the module's own forward."""
     torch = _torch()
     x, mask, angles = kwargs.get("hidden_states"), kwargs.get("attention_mask"), kwargs.get("position_embeddings")
     if (args or x is None or x.dim() != 3 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16)
-            or (mask is not None and mask.dtype != torch.int32) or not isinstance(angles, _Angles) or angles.table.head_dim != self.head_dim or self.head_dim % 8 or self.head_dim > 256):
+            or _drops(self) or (mask is not None and mask.dtype != torch.int32) or not isinstance(angles, _Angles) or angles.table.head_dim != self.head_dim or self.head_dim % 8 or self.head_dim > 256):
         return self._mv_attn_forward(*args, **kwargs)
     batch, rows = x.shape[:2]
     q, k, v = (proj(x).view(batch, rows, -1, self.head_dim) for proj in (self.q_proj, self.k_proj, self.v_proj))
@@ -565,7 +570,7 @@ def _packed_forward(self, hidden_states, *args, **kwargs):
     torch = _torch()
     x, offsets, angles = hidden_states, kwargs.get("cu_seqlens"), kwargs.get("position_embeddings")
     dim = self.head_dim
-    if (args or x.dim() != 2 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16) or offsets is None or angles is None
+    if (args or x.dim() != 2 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16) or _drops(self) or offsets is None or angles is None
             or offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.device != x.device or angles[0].dtype != torch.float32
             or angles[0].shape != (x.shape[0], dim) or dim % 8 or dim > 256):
         return self._mv_attn_forward(hidden_states, *args, **kwargs)
@@ -590,7 +595,7 @@ def patch_attention(model: Any) -> Dict[str, int]:
     """Run the attention of a transformers encoder through this module, in place: the model's attention function becomes `attention` (with the mask
     of a forward as key ranges), its decoder blocks rotate by positions, its packed vision blocks attend all documents and windows in one launch (the
     framework takes them one by one).  Modules fall back to their own forward for anything the kernels do not take (not on a GPU, autograd on, another
-    type, a mask with holes).  -> modules patched per kind.  `unpatch_attention` undoes it."""
+    type, a mask with holes, dropout of a model in training mode).  -> modules patched per kind.  `unpatch_attention` undoes it."""
     from transformers import AttentionInterface, AttentionMaskInterface
 
     counts = {"rotary": 0, "decoder": 0, "packed": 0}

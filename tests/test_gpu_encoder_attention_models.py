@@ -75,3 +75,24 @@ def test_without_a_mask_the_forward_then_the_module_say_whether_rows_are_causal(
             for asked in (None, True, False):
                 got = ea._interface_attention(module, q, k, v, is_causal=asked)[0]
                 assert near(got, AttentionInterface()["sdpa"](module, q, k, v, None, is_causal=asked)[0])
+
+
+def test_dropout_of_a_model_in_training_mode_stays(ea):
+    """Under no_grad too: the same bits as the unpatched model from the same random state; in evaluation mode the kernels run again."""
+    x = ids()
+    padded = torch.ones_like(x)
+    padded[1, 5:] = 0
+    model = gemma(attention_dropout=0.5).train()
+
+    def run(seed, mask):
+        torch.manual_seed(seed)
+        with torch.no_grad():
+            return model(input_ids=x, attention_mask=mask).last_hidden_state
+
+    plain = [run(s, m) for s in (1, 2) for m in (None, padded)]
+    ea.patch_attention(model)
+    got = [run(s, m) for s in (1, 2) for m in (None, padded)]
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[2], plain[2]) and not near(got[0], got[2])
+    assert all(near(a[padded.bool()], b[padded.bool()]) for a, b in zip(got, plain))
+    model.eval()
+    assert not near(run(1, None), plain[0]) and torch.equal(run(1, None), run(2, None))

@@ -537,13 +537,18 @@ def _rotary_forward(self, x, position_ids, *args, **kwargs):
     return out
 
 
+def _ours(torch, *projections) -> bool:
+    """Whether what the projections return is this block's to overwrite: a plain linear layer's new tensor, which no hook has been handed."""
+    return not torch.nn.modules.module._global_forward_hooks and all(type(p) is torch.nn.Linear and not p._forward_hooks for p in projections)
+
+
 def _drops(module) -> bool:
     """Training mode (under no_grad) with dropout of the attention's weights: not in the kernel."""
     return bool(module.training and getattr(module, "attention_dropout", 0.0))
 
 
 def _decoder_forward(self, *args, **kwargs):
-    """q, k, v -> rotation in place -> attention over key ranges -> output projection; what does not fit goes through the module's own forward."""
+    """q, k, v -> rotation (in place where they are the block's own) -> attention over key ranges -> output projection; what does not fit goes through the module's own forward."""
     torch = _torch()
     x, mask, angles = kwargs.get("hidden_states"), kwargs.get("attention_mask"), kwargs.get("position_embeddings")
     if (args or x is None or x.dim() != 3 or not x.is_cuda or torch.is_grad_enabled() or x.dtype not in (torch.bfloat16, torch.float16)
@@ -551,7 +556,7 @@ def _decoder_forward(self, *args, **kwargs):
         return self._mv_attn_forward(*args, **kwargs)
     batch, rows = x.shape[:2]
     q, k, v = (proj(x).view(batch, rows, -1, self.head_dim) for proj in (self.q_proj, self.k_proj, self.v_proj))
-    q, k = rotary(q, k, angles.positions, angles.table, in_place=True)
+    q, k = rotary(q, k, angles.positions, angles.table, in_place=_ours(torch, self.q_proj, self.k_proj))
     cache = kwargs.get("past_key_values")
     if cache is not None:
         k, v = (t.transpose(1, 2) for t in cache.update(k.transpose(1, 2), v.transpose(1, 2), self.layer_idx))
@@ -566,7 +571,7 @@ def _decoder_forward(self, *args, **kwargs):
 
 
 def _packed_forward(self, hidden_states, *args, **kwargs):
-    """Packed patches: fused projection -> rotation by the tower's tables, in place -> attention within each document or window -> output projection."""
+    """Packed patches: fused projection -> rotation by the tower's tables (as above) -> attention within each document or window -> output projection."""
     torch = _torch()
     x, offsets, angles = hidden_states, kwargs.get("cu_seqlens"), kwargs.get("position_embeddings")
     dim = self.head_dim
@@ -576,7 +581,7 @@ def _packed_forward(self, hidden_states, *args, **kwargs):
         return self._mv_attn_forward(hidden_states, *args, **kwargs)
     q, k, v = self.qkv(x).view(x.shape[0], 3, -1, dim).unbind(1)
     cos, sin = (t[:, : dim // 2] for t in angles)
-    q, k = rotary_tables(q, k, cos, sin, in_place=True)
+    q, k = rotary_tables(q, k, cos, sin, in_place=_ours(torch, self.qkv))
     out = attention(q, k, v, key_ranges=document_ranges(offsets, x.shape[0]), scale=self.scaling)
     return self.proj(out.flatten(1))
 

@@ -96,3 +96,43 @@ def test_dropout_of_a_model_in_training_mode_stays(ea):
     assert all(near(a[padded.bool()], b[padded.bool()]) for a, b in zip(got, plain))
     model.eval()
     assert not near(run(1, None), plain[0]) and torch.equal(run(1, None), run(2, None))
+
+
+@pytest.mark.parametrize("how", ["module", "global", "wrapped"])
+def test_what_a_projection_returned_stays_as_it_was(ea, how):
+    """A forward hook that keeps the outputs of q_proj and k_proj sees the projections, not their rotated values; so does a layer that keeps its own output."""
+    kept = {}
+
+    def keep(module, args, out):
+        if isinstance(module, torch.nn.Linear):
+            kept[module] = (args[0], out)
+
+    class Keeping(torch.nn.Linear):
+        def forward(self, x):
+            out = super().forward(x)
+            keep(self, (x,), out)
+            return out
+
+    model, x = gemma(), ids()
+    with torch.inference_mode():
+        ea.patch_attention(model)
+        want = model(input_ids=x).last_hidden_state
+        blocks = [layer.self_attn for layer in model.layers]
+        handles = []
+        if how == "module":
+            handles = [p.register_forward_hook(keep) for b in blocks for p in (b.q_proj, b.k_proj)]
+        elif how == "global":
+            handles = [torch.nn.modules.module.register_module_forward_hook(keep)]
+        else:
+            for b in blocks:
+                for p in (b.q_proj, b.k_proj):
+                    p.__class__ = Keeping
+        try:
+            assert torch.equal(model(input_ids=x).last_hidden_state, want)
+        finally:
+            for h in handles:
+                h.remove()
+        for b in blocks:
+            for p in (b.q_proj, b.k_proj):
+                seen, out = kept[p]
+                assert torch.equal(out, torch.nn.functional.linear(seen, p.weight, p.bias))

@@ -523,12 +523,14 @@ def _rotary_forward(self, x, position_ids, *args, **kwargs):
     angles = self._mv_attn_forward(x, position_ids, *args, **kwargs)
     if not x.is_cuda or torch.is_grad_enabled() or position_ids.dtype not in (torch.int32, torch.int64) or position_ids.dim() not in (2, 3):
         return angles
-    table = self._mv_rotary_table
-    if table is None or table.inv_freq.device != x.device:
+    freq, scale = self.inv_freq, float(getattr(self, "attention_scaling", 1.0))
+    made_of = (freq, None if freq.is_inference() else freq._version, scale, x.device)  # a model that is cast or moved gets new frequencies
+    kept = self._mv_rotary_table
+    if kept is None or kept[0][0] is not freq or kept[0][1:] != made_of[1:]:
         sections = self._mv_rotary_sections
         axes = None if sections is None else [a for a, n in enumerate(sections) for _ in range(n)]
-        table = self._mv_rotary_table = RotaryTable(self.inv_freq, axes, head_dim=2 * int(self.inv_freq.shape[0]), scale=float(getattr(self, "attention_scaling", 1.0)),
-                                                    device=x.device)
+        kept = self._mv_rotary_table = made_of, RotaryTable(freq, axes, head_dim=2 * int(freq.shape[0]), scale=scale, device=x.device)
+    table = kept[1]
     positions = position_ids[None] if position_ids.dim() == 2 else position_ids
     if positions.shape[0] < table.axes:
         return angles

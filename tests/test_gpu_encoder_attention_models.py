@@ -136,3 +136,44 @@ def test_what_a_projection_returned_stays_as_it_was(ea, how):
             for p in (b.q_proj, b.k_proj):
                 seen, out = kept[p]
                 assert torch.equal(out, torch.nn.functional.linear(seen, p.weight, p.bias))
+
+
+def test_frequencies_that_change_after_the_first_forward_are_used(ea):
+    """Assigned anew, changed in place, cast with the model, another attention_scaling: each forward turns by what the rotary module holds then."""
+    model, plain, x = gemma(), gemma(), ids(rows=60)
+    for m in (model, plain):
+        for layer in m.layers:  # scores of about 1: of the random weights as they are every row is nearly the mean of its keys, however it is turned
+            layer.self_attn.q_proj.weight.data *= 5
+            layer.self_attn.k_proj.weight.data *= 5
+    ea.patch_attention(model)
+
+    def assign(m):
+        m.rotary_emb.inv_freq = m.rotary_emb.inv_freq * 3
+
+    def in_place(m):
+        m.rotary_emb.inv_freq.mul_(0.2)
+
+    def scaling(m):
+        m.rotary_emb.attention_scaling = 0.5
+
+    def cast(m):
+        m.to(torch.float16)
+
+    with torch.inference_mode():
+        last = model(input_ids=x).last_hidden_state
+        for change in (assign, scaling):
+            change(model), change(plain)
+            got, want = model(input_ids=x).last_hidden_state, plain(input_ids=x).last_hidden_state
+            assert near(got, want) and not near(got, last), change.__name__
+            last = got
+    for change in (in_place, cast):
+        with torch.no_grad():
+            model.rotary_emb.inv_freq, plain.rotary_emb.inv_freq = (torch.arange(16, 0, -1, device="cuda") / 7.0 for _ in range(2))
+            model(input_ids=x)
+            change(model), change(plain)
+            got, want = model(input_ids=x).last_hidden_state, plain(input_ids=x).last_hidden_state
+            assert near(got, want), change.__name__
+    table = model.rotary_emb._mv_rotary_table
+    with torch.no_grad():
+        model(input_ids=x)
+    assert model.rotary_emb._mv_rotary_table is table  # and not made again where nothing changed

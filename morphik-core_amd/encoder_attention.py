@@ -30,6 +30,7 @@ from . import _lib
 
 _PAIRINGS = ("halves", "adjacent")
 _FP32_MAX = 2.0**128 - 2.0**104
+_MAX_ROW_STRIDE = 1 << 23  # of k and v, in elements
 _FORMATS = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
 
 
@@ -402,7 +403,7 @@ def attention(q: Any, k: Any, v: Any, *, key_ranges: Any = None, causal: bool = 
     a multiple of kv_heads.  key_ranges int32 [batch or 1, rows, 2]: row i sees the keys [lo, hi), cut to what there is; an empty range gives
     zeros; None: every key, or with `causal` those up to the row itself (the last row stands at the last key).  scale defaults to dim ** -0.5; softcap
     c > 0 caps scores to c * tanh(score / c).  bfloat16 or float16; dim a multiple of 8 up to 256; any strides that are multiples of 8 with the elements
-    of a head side by side, 16-byte aligned.
+    of a head side by side, 16-byte aligned, rows of k and v at most 2^23 elements apart.
     -> new contiguous tensor of q's shape."""
     torch = _torch()
     what = "attention"
@@ -472,13 +473,21 @@ def enabled_by_env() -> bool:
     return os.environ.get("MV_ENCODER_FUSED_ATTENTION", "0") in ("1", "true", "yes")
 
 
-def _kernel_takes(torch, *tensors) -> bool:
-    """Inference on a GPU in a type and layout that `attention` has; anything else goes the framework's way."""
-    first = tensors[0]
-    if not first.is_cuda or torch.is_grad_enabled() or first.dtype not in (torch.bfloat16, torch.float16) or first.shape[-1] % 8 or not 8 <= first.shape[-1] <= 256:
+def _kernel_takes(torch, query, key, value, scaling=None, softcap=None) -> bool:
+    """Inference on a GPU in types, shapes and a layout ([batch, heads, rows, dim]) that `attention` has; anything else goes the framework's way."""
+    return query.is_cuda and not torch.is_grad_enabled() and _fits(torch, query, key, value, scaling, softcap)
+
+
+def _fits(torch, query, key, value, scaling=None, softcap=None) -> bool:
+    dtype, device, dim = query.dtype, query.device, query.shape[-1]
+    if dtype not in (torch.bfloat16, torch.float16) or dim % 8 or not 8 <= dim <= 256 or key.shape != value.shape or key.shape[0] != query.shape[0] or key.shape[3] != dim:
         return False
-    return all(t.dtype == first.dtype and t.device == first.device and t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(st % 8 for st in t.stride()[:-1])
-               for t in tensors)
+    if key.shape[1] < 1 or query.shape[1] < 1 or query.shape[1] % key.shape[1] or max(key.stride(2), value.stride(2)) > _MAX_ROW_STRIDE:
+        return False
+    scale, cap = dim**-0.5 if scaling is None else scaling, softcap or 0.0
+    if not 0 < scale * 4 < _FP32_MAX or not 0 <= cap * 4 < _FP32_MAX or cap and not 1e-36 < scale / cap < 1e36:
+        return False
+    return all(t.dtype == dtype and t.device == device and t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(st % 8 for st in t.stride()[:-1]) for t in (query, key, value))
 
 
 def _is_causal(module, asked: Optional[bool]) -> bool:
@@ -493,7 +502,7 @@ def _interface_attention(module, query, key, value, attention_mask=None, scaling
     causal = attention_mask is None and query.shape[2] > 1 and _is_causal(module, is_causal)
     known = ranges is not None or attention_mask is None and not (causal and query.shape[2] != key.shape[2])
     extras = any(kwargs.get(name) is not None for name in ("s_aux", "position_bias"))  # sinks, added biases: not in the kernel
-    if known and not dropout and not extras and _kernel_takes(torch, query, key, value):
+    if known and not dropout and not extras and _kernel_takes(torch, query, key, value, scaling, softcap):
         out = attention(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), key_ranges=ranges, causal=causal, scale=scaling, softcap=softcap or 0.0)
         return out, None
     from transformers import AttentionInterface
@@ -561,7 +570,11 @@ def _decoder_forward(self, *args, **kwargs):
     q, k = rotary(q, k, angles.positions, angles.table, in_place=_ours(torch, self.q_proj, self.k_proj))
     cache = kwargs.get("past_key_values")
     if cache is not None:
-        k, v = (t.transpose(1, 2) for t in cache.update(k.transpose(1, 2), v.transpose(1, 2), self.layer_idx))
+        heads_first = q.transpose(1, 2), *cache.update(k.transpose(1, 2), v.transpose(1, 2), self.layer_idx)
+        if not _kernel_takes(torch, *heads_first, self.scaling):  # what a cache hands back may be of another type or layout
+            out, _ = _interface_attention(self, *heads_first, mask, scaling=self.scaling, is_causal=kwargs.get("is_causal"))
+            return self.o_proj(out.flatten(2)), None
+        k, v = (t.transpose(1, 2) for t in heads_first[1:])
     if mask is not None:
         out = attention(q, k, v, key_ranges=mask[:, 0], scale=self.scaling)
     else:

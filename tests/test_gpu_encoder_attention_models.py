@@ -177,3 +177,30 @@ def test_frequencies_that_change_after_the_first_forward_are_used(ea):
     with torch.no_grad():
         model(input_ids=x)
     assert model.rotary_emb._mv_rotary_table is table  # and not made again where nothing changed
+
+
+def test_calls_that_the_kernel_does_not_take_fall_back(ea):
+    """Values of another width than the keys, rows of K further apart than the kernel reaches, a cache that hands back another layout: the framework's function
+    answers, where `attention` itself refuses."""
+    from transformers import AttentionInterface, DynamicCache
+
+    class Module(torch.nn.Module):
+        is_causal = False
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(1, h, n, d, generator=g, device="cuda").to(torch.bfloat16) for h, n, d in ((2, 5, 32), (2, 3, 32), (2, 3, 16)))
+    far = torch.zeros(2 * (1 << 23) + 4096, dtype=torch.bfloat16, device="cuda").as_strided((1, 2, 2, 32), (64, 32, (1 << 23) + 8, 1))
+    far.copy_(k[:, :, :2])
+    with torch.inference_mode():
+        for args in ((q, k, v), (q, far, far), (q, far, k[:, :, :2])):
+            got = ea._interface_attention(Module(), *args)[0]
+            assert near(got, AttentionInterface()["sdpa"](Module(), *args, None)[0])
+
+        class Odd(DynamicCache):
+            def update(self, *args, **kwargs):
+                return tuple(torch.nn.functional.pad(t, (0, 4))[..., :-4] for t in super().update(*args, **kwargs))
+
+        model, x = gemma(), ids()
+        want = model(input_ids=x).last_hidden_state
+        ea.patch_attention(model)
+        assert near(model(input_ids=x, past_key_values=Odd(config=model.config), use_cache=True).last_hidden_state, want)

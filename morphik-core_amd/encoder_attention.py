@@ -490,6 +490,21 @@ def _fits(torch, query, key, value, scaling=None, softcap=None) -> bool:
     return all(t.dtype == dtype and t.device == device and t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(st % 8 for st in t.stride()[:-1]) for t in (query, key, value))
 
 
+def _capped_attention(torch, module, query, key, value, mask, scaling, dropout, softcap, causal):
+    """The formula of `attention` in plain operations, in 32 bits: capped scores where the kernel does not apply."""
+    group, rows, keys = query.shape[1] // key.shape[1], query.shape[2], key.shape[2]
+    k, v = (t.float().repeat_interleave(group, 1) for t in (key, value))
+    s = torch.matmul(query.float(), k.transpose(2, 3).contiguous()) * (query.shape[3] ** -0.5 if scaling is None else scaling)
+    s = softcap * torch.tanh(s / softcap)
+    if causal:
+        mask = torch.ones(rows, keys, dtype=torch.bool, device=query.device).tril()
+    if mask is not None:
+        s = s.masked_fill(~mask, -math.inf) if mask.dtype == torch.bool else s + mask
+    p = torch.softmax(s, -1).masked_fill((s == -math.inf).all(-1, keepdim=True), 0.0)  # a row that sees nothing is zero
+    p = torch.nn.functional.dropout(p, dropout, module.training)
+    return torch.matmul(p, v).to(query.dtype).transpose(1, 2).contiguous()
+
+
 def _is_causal(module, asked: Optional[bool]) -> bool:
     """Without a mask: what the forward asks for, else what the module says; one that says nothing is causal, as the framework's own function takes it."""
     return bool(getattr(module, "is_causal", True) if asked is None else asked)
@@ -510,6 +525,10 @@ def _interface_attention(module, query, key, value, attention_mask=None, scaling
     if ranges is not None:  # back to a boolean mask
         at = torch.arange(key.shape[2], device=query.device, dtype=torch.int32)
         attention_mask = ((at >= ranges[..., :1]) & (at < ranges[..., 1:]))[:, None]
+    if softcap:  # the framework's function has none
+        if extras:
+            raise ValueError("attention: a softcap together with sinks or an added bias")
+        return _capped_attention(torch, module, query, key, value, attention_mask, scaling, dropout, softcap, causal), None
     return AttentionInterface()["sdpa"](module, query, key, value, attention_mask, scaling=scaling, dropout=dropout, is_causal=is_causal, **kwargs)
 
 

@@ -42,3 +42,34 @@ def test_what_the_kernel_refuses_goes_the_frameworks_way():
         assert not ea._fits(torch, *args), [tuple(t.shape) for t in args]
     for scaling, cap in ((0.0, 0.0), (-1.0, 0.0), (float("nan"), 0.0), (float("inf"), 0.0), (3e38, 0.0), (1.0, -1.0), (1.0, 3e38), (1.0, float("nan")), (1e-30, 1e30), (3e38, 1e-3)):
         assert not ea._fits(torch, q, k, k, scaling, cap), (scaling, cap)
+
+
+def test_a_softcap_is_kept_where_the_kernel_does_not_apply():
+    """Off the GPU, and with a mask of holes: the capped formula in 64 bits, not the framework's uncapped function.  32-bit sums over 16 and 7 terms: 1e-5."""
+
+    class Module(torch.nn.Module):
+        num_key_value_groups = 2
+
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(2, h, 7, 16, generator=g) * x for h, x in ((4, 6.0), (2, 2.0), (2, 1.0)))
+    bits = torch.rand(2, 1, 7, 7, generator=g) < 0.6
+    bits[:, :, 3] = False
+    low = torch.where(bits, 0.0, torch.finfo(torch.float32).min)
+    below = torch.ones(7, 7, dtype=torch.bool).tril()[None, None].expand(2, 1, 7, 7)
+    r = torch.tensor([[[0, 4], [1, 3], [2, 2], [0, 7], [5, 7], [0, 1], [3, 7]]] * 2, dtype=torch.int32)
+    at = torch.arange(7)
+    runs = ((at >= r[..., :1]) & (at < r[..., 1:]))[:, None]
+    for mask, seen, kw in ((None, below, {}), (None, torch.ones_like(below), dict(is_causal=False)), (bits, bits, {}), (low, bits, {}), (r[:, None], runs, {})):
+        s = 5.0 * torch.tanh(q.double() @ k.double().repeat_interleave(2, 1).transpose(2, 3) * 0.25 / 5.0)
+        s = s.masked_fill(~seen, -torch.inf)
+        p = torch.softmax(s, -1).nan_to_num(0.0)
+        want = (p @ v.double().repeat_interleave(2, 1)).transpose(1, 2)
+        got = ea._interface_attention(Module(), q, k, v, mask, scaling=0.25, softcap=5.0, **kw)[0]
+        if mask is low:  # every key of an all-masked row weighs the same there
+            got, want = (t[:, [0, 1, 2, 4, 5, 6]] for t in (got, want))
+        assert torch.allclose(got.double(), want, rtol=0, atol=1e-5)
+    with pytest.raises(ValueError, match="softcap"):
+        ea._interface_attention(Module(), q, k, v, None, softcap=5.0, position_bias=low)
+    x = q.clone().requires_grad_()
+    ea._interface_attention(Module(), x, k, v, bits, softcap=5.0)[0].sum().backward()
+    assert bool(torch.isfinite(x.grad).all())

@@ -234,22 +234,44 @@ def _overlaps(x) -> bool:
 
 
 def _share_memory(a, b) -> bool:
-    """Conservative but for views of one buffer whose heads lie side by side in its rows (a fused projection)."""
+    """Conservative, but not for parts of one buffer: heads side by side in its rows (a fused projection), whatever the order of its dimensions."""
     if not a.numel() or not b.numel():
         return False
     (a0, a1), (b0, b1) = _extent(a), _extent(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    if a.stride()[:2] == b.stride()[:2]:
+    lo, hi = (a, b) if a0 <= b0 else (b, a)
+    gap, rest = divmod(hi.data_ptr() - lo.data_ptr(), a.element_size())
+    if rest:
+        return True
+    if a.stride()[:2] == b.stride()[:2] and a.shape[:2] == b.shape[:2]:
         # the same rows of one buffer: apart if their windows within a row's step do not meet, seen from the lower one
-        size = a.element_size()
-        lo, hi = (a, b) if a0 <= b0 else (b, a)
-        gap = (hi.data_ptr() - lo.data_ptr()) // size
         width = [1 + sum((n - 1) * st for n, st in zip(x.shape[2:], x.stride()[2:])) for x in (lo, hi)]
-        step = min((st for st, n in zip(a.stride()[:2], a.shape[:2]) if n > 1), default=None)
-        if gap >= width[0] and (step is None or gap + width[1] <= step):
+        outer = sorted((st, n) for st, n in zip(a.stride()[:2], a.shape[:2]) if n > 1)
+        nearest = min((st for st, _ in outer), default=None)  # of two rows' starts
+        if len(outer) == 2:
+            nearest = min(nearest, outer[1][0] - outer[0][0] * (outer[0][1] - 1))
+        if gap >= width[0] and (nearest is None or gap + width[1] <= nearest):
             return False
-    return True
+    # boxes of one grid: with the same steps, `hi` starts some whole steps from `lo` in each dimension; where the box that holds both steps past itself, two
+    # elements share memory only if all their places are the same, so one dimension in which the boxes do not meet is enough
+    steps = []
+    for st_l, n_l, st_h, n_h in zip(lo.stride(), lo.shape, hi.stride(), hi.shape):
+        if n_l > 1 and n_h > 1 and st_l != st_h:
+            return True
+        if max(n_l, n_h) > 1:
+            steps.append((st_l if n_l > 1 else st_h, n_l, n_h))
+    reach, apart, left = 0, False, gap
+    boxes = []
+    for st, n_l, n_h in sorted(steps, reverse=True):
+        at, left = divmod(left, st) if st else (0, left)
+        boxes.append((st, max(n_l, at + n_h)))
+        apart |= at >= n_l
+    for st, n in reversed(boxes):
+        if n > 1 and st <= reach:
+            return True
+        reach += st * (n - 1)
+    return left != 0 or not apart
 
 
 def rotary(q: Any, k: Any, positions: Any, table: RotaryTable, *, in_place: bool = False) -> Tuple[Any, Any]:

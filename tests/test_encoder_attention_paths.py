@@ -73,3 +73,46 @@ def test_a_softcap_is_kept_where_the_kernel_does_not_apply():
     x = q.clone().requires_grad_()
     ea._interface_attention(Module(), x, k, v, bits, softcap=5.0)[0].sum().backward()
     assert bool(torch.isfinite(x.grad).all())
+
+
+def test_parts_of_one_buffer_are_told_from_parts_that_overlap():
+    """Against the places themselves: pairs of slices, in the order of a projection and with the heads outside the rows, of one batch entry and several, cut
+    along any dimension.  Never apart where an element is in both; heads cut from a buffer apart, in either order of its dimensions."""
+    import itertools
+    import random
+
+    def places(t):
+        index = torch.zeros((), dtype=torch.int64)
+        for st, n in zip(t.stride(), t.shape):
+            index = index[..., None] + st * torch.arange(n)
+        return set((index + t.storage_offset()).flatten().tolist())
+
+    rng = random.Random(1)
+    told = 0
+    for batch, heads_outside in itertools.product((1, 3), (False, True)):
+        rows, heads, dim = 5, 6, 4
+        whole = torch.zeros(batch, heads, rows, dim).transpose(1, 2) if heads_outside else torch.zeros(batch, rows, heads, dim)
+        q, k, v = whole.split([3, 1, 2], 2)
+        for a, b in itertools.permutations((q, k, v), 2):
+            assert not ea._share_memory(a, b)
+        for _ in range(600):
+            parts = []
+            for _ in range(2):
+                t = whole
+                for d in range(4):
+                    lo = rng.randrange(t.shape[d])
+                    hi = rng.randrange(lo, t.shape[d]) + 1
+                    t = t.narrow(d, lo, hi - lo) if rng.random() < 0.6 else t
+                parts.append(t)
+            meet = bool(places(parts[0]) & places(parts[1]))
+            said = ea._share_memory(*parts)
+            assert said or not meet
+            assert said == ea._share_memory(*parts[::-1])
+            told += not meet and not said
+    assert told > 300
+    flat = torch.zeros(400)
+    for _ in range(2000):  # any two strided boxes of one buffer
+        parts = [flat.as_strided([rng.randint(1, 3) for _ in range(4)], [rng.randint(0, 40) for _ in range(3)] + [1], rng.randint(0, 60)) for _ in range(2)]
+        assert ea._share_memory(*parts) or not places(parts[0]) & places(parts[1])
+    near = [flat.as_strided((2, 3, 1, 4), (24, 10, 4, 1), at) for at in (0, 5)]  # the second entry's first row starts 4 behind the first one's last
+    assert places(near[0]) & places(near[1]) and ea._share_memory(*near)

@@ -166,3 +166,15 @@ def test_forward_mode_tangents_are_refused(ea):  # noqa: F811
         with pytest.raises(ValueError, match="tangent"):
             ea.rotary_tables(q, k, cos, forward_ad.make_dual(cos, torch.ones_like(cos)))
         assert ea.attention(q, k, v).shape == q.shape and ea.rotary(q, k, pos, table)[0].shape == q.shape
+
+
+def test_heads_of_one_buffer_outside_the_rows_turn_in_place(ea):  # noqa: F811
+    """q and k as parts of one [batch, heads, rows, dim] buffer: the bits of a new tensor, the heads behind them as they were."""
+    g = gen(44)
+    whole = torch.randn(3, 8, 11, 64, generator=g, device="cuda").to(torch.bfloat16)
+    keep = whole.clone()
+    q, k = whole[:, :4].transpose(1, 2), whole[:, 4:6].transpose(1, 2)
+    table, pos = ea.RotaryTable.with_sections(64, [32]), torch.arange(11, device="cuda")
+    want = ea.rotary(q, k, pos, table)
+    a, b = ea.rotary(q, k, pos, table, in_place=True)
+    assert a is q and b is k and torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(whole[:, 6:], keep[:, 6:])

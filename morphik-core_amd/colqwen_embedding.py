@@ -119,12 +119,9 @@ class MI355XColQwen2EmbeddingModel(BaseEmbeddingModel):
             if fused_ops or encoder_ops.enabled_by_env():
                 self.fused_ops = encoder_ops.patch_encoder(self.model)
         # rotary positions and attention as HIP kernels (encoder_attention.py): on request, or where MV_ENCODER_FUSED_ATTENTION=1
-        self.fused_attention = {"rotary": 0, "decoder": 0, "packed": 0}
-        if self.device.type == "cuda" and fused_attention is not False:
-            from . import encoder_attention
+        from . import encoder_attention
 
-            if fused_attention or encoder_attention.enabled_by_env():
-                self.fused_attention = encoder_attention.patch_attention(self.model)
+        self.fused_attention = encoder_attention.patch_on_request(self.model, self.device, fused_attention)
 
     # ------------------------------------------------------------------ forward
     def _forward(self, batch) -> Tuple[Any, Any]:

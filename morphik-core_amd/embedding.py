@@ -140,12 +140,9 @@ class MI355XColpaliEmbeddingModel(BaseEmbeddingModel):
                 self.fused_ops = encoder_ops.patch_encoder(self.model)
             # GEMM solutions tuned for this architecture's shapes on an MI355X (ignored by PyTorch on any other stack)
             self.tuned_gemms = encoder_ops.load_tuned_gemms()
-        self.fused_attention = {"rotary": 0, "decoder": 0, "packed": 0}
-        if self.device.type == "cuda" and fused_attention is not False:
-            from . import encoder_attention
+        from . import encoder_attention
 
-            if fused_attention or encoder_attention.enabled_by_env():
-                self.fused_attention = encoder_attention.patch_attention(self.model)
+        self.fused_attention = encoder_attention.patch_on_request(self.model, self.device, fused_attention)
         cfg = self.model.config.vlm_config
         self.image_size = int(cfg.vision_config.image_size)
         self.n_image_tokens = (self.image_size // int(cfg.vision_config.patch_size)) ** 2

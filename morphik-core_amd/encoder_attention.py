@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import logging
 import math
 import os
 import struct
@@ -27,6 +28,8 @@ import types
 from typing import Any, Dict, Optional, Sequence, Tuple
 
 from . import _lib
+
+logger = logging.getLogger(__name__)
 
 _PAIRINGS = ("halves", "adjacent")
 _FP32_MAX = 2.0**128 - 2.0**104
@@ -686,6 +689,17 @@ def patch_attention(model: Any) -> Dict[str, int]:
         mod.forward = types.MethodType(forward, mod)
         counts[kind] += 1
     return counts
+
+
+def patch_on_request(model: Any, device: Any, asked: Optional[bool]) -> Dict[str, int]:
+    """The `fused_attention=` option of the embedding models: True, or None with MV_ENCODER_FUSED_ATTENTION=1, patches a model on a GPU.  There are no kernels
+    anywhere else: a request by name is answered by a warning there.  -> modules patched per kind"""
+    if asked is not False and (asked or enabled_by_env()):
+        if device.type == "cuda":
+            return patch_attention(model)
+        if asked:
+            logger.warning("fused_attention: the model is on %s, its attention stays the framework's (the kernels need a GPU)", device)
+    return {"rotary": 0, "decoder": 0, "packed": 0}
 
 
 def unpatch_attention(model: Any) -> None:

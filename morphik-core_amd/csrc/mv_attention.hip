@@ -166,6 +166,7 @@ __device__ uint32_t spoiled_rows(const AttnArgs& a, const uint16_t* q, const uin
     const int from = min(max(lo - k0, 0), 64), to = min(max(hi - k0, 0), 64);
     const uint64_t sees = from < to ? ~0ull >> (64 - (to - from)) << from : 0;
     hit |= ((odds & ~sees) | (infs & sees)) != 0;
+    if (k0 + BK > k_hi) hit |= odds >> (k_hi - 1 - k0) & 1;  // the rows behind the last key are copies of it, under weights of 0
     if (CAP != kNoCap) continue;  // a cap makes every infinite score finite
     for (uint64_t left = infs; left; left &= left - 1) {
       const int at = __builtin_ctzll(left);
@@ -208,6 +209,10 @@ __device__ void exact_rows(const AttnArgs& a, const AgainRow (&rows)[R], int cou
     from = min(from, rows[r].lo), to = max(to, rows[r].hi);
   }
   for (int j0 = from; j0 < to; j0 += 64) {
+    bool any = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) any |= rows[r].lo < j0 + 64 && rows[r].hi > j0;
+    if (!any) continue;
     const int n = min(to - j0, 64), j = j0 + lane;
     const uint16_t* kr = k + (int64_t)(j0 + min(lane, n - 1)) * a.k_l;
     float s[R] = {};

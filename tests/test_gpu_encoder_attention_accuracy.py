@@ -178,3 +178,22 @@ def test_heads_of_one_buffer_outside_the_rows_turn_in_place(ea):  # noqa: F811
     want = ea.rotary(q, k, pos, table)
     a, b = ea.rotary(q, k, pos, table, in_place=True)
     assert a is q and b is k and torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(whole[:, 6:], keep[:, 6:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [72, 128])
+@pytest.mark.parametrize("rows,keys", [(3, 1), (40, 70), (4, 2501), (64, 128)])
+def test_an_infinite_value_at_the_last_key_is_infinite(ea, dtype, dim, rows, keys):  # noqa: F811
+    """The last key of a call that ends inside a tile: its column is infinite in the rows that see it, not NaN, and no row's other columns change."""
+    g = gen(keys)
+    q, k, v = (make(g, 1, n, 2, dim, DT[dtype], "split", x) for n, x in ((rows, 0.3), (keys, 1.0), (keys, 1.0)))
+    r = torch.tensor([0, keys], dtype=torch.int32, device="cuda").repeat(1, rows, 1)
+    r[:, 1::2, 1] -= 1  # every other row ends in front of it
+    want, tol = ranges_oracle(q, k, v, r)
+    for x in (math.inf, -math.inf):
+        v2 = v.clone()
+        v2[:, -1, :, 3] = x
+        got = ea.attention(q, k, v2, key_ranges=r)
+        assert bool((got[:, ::2, :, 3] == x).all())
+        got[:, ::2, :, 3] = want[:, ::2, :, 3].to(got.dtype)
+        check(got, want, tol + 2.0**-7 * want.abs(), x)

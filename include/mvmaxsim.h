@@ -497,10 +497,12 @@ MV_API int mv_enc_rotary(int device, const mv_rotary* p, void* stream);
  *                  ranges[b][i][0] <= j < ranges[b][i][1] (cut to 0 .. keys; an empty range gives zeros; ranges NULL: every key, or
  *                  with causal != 0 those up to the row itself, the last row standing at the last key).
  *                  softcap c > 0: scores become c * tanh(score / c) first.  What keys outside a row's range hold does not reach the row,
- *                  NaN and infinity included; a column that holds an infinite value a row sees is infinite (NaN where its weight rounds to 0).  dtype MV_BF16 or MV_F16; dim a multiple of 8 up to 256; pointers 16-byte aligned (ranges: 8),
- *                  strides multiples of 8 (ranges: 2, 0 = one for all); out contiguous [batch][rows][heads][dim].  Sums and softmax statistics
- *                  are held in 32 bits, weights rounded to dtype for the product with v (in fp16 at most 2^-36 of a row's sum is lost a key).  Rows of k and v at most 2^23 elements apart.  Calls too small to
- *                  fill the card are cut along the keys: their 32-bit sums pass through `workspace` and a second kernel joins them. */
+ *                  NaN and infinity included; a column that holds an infinite value a row sees is infinite (NaN where its weight rounds to 0).
+ *                  dtype MV_BF16 or MV_F16; dim a multiple of 8 up to 256; pointers 16-byte aligned (ranges: 8), strides multiples of 8
+ *                  (ranges: 2, 0 = one for all); rows of k and v at most 2^23 elements apart; out contiguous [batch][rows][heads][dim].  Sums and
+ *                  softmax statistics are held in 32 bits (bf16 values past 2^120 / keys may overflow them), weights rounded to dtype for the product
+ *                  with v (in fp16 at most 2^-36 of a row's sum is lost a key).  Calls too small to fill the card are cut along the keys: their
+ *                  32-bit sums pass through `workspace` and a second kernel joins them. */
 typedef struct mv_attn {
   const void *q, *k, *v;
   void* out;

@@ -35,8 +35,8 @@ using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaveRows = 32;                  // rows of a wave: the N of the 32x32x16 matrix instruction
 constexpr int kXcds = 8;
-// By KC, the 16-column steps of a head.  Keys of a tile: two products deep where the registers allow it.  Waves of a SIMD at once: by registers; heads of
-// 72 ... 96 would fit three, which is slower (8464 rows of heads of 80: 444 us with two, 475 with three).
+// By KC, the 16-column steps of a head.  Keys of a tile: two products deep where the registers allow it.  Waves of a SIMD at once: by registers.  Three
+// would have 168 each of the 190 ... 200 that heads of 72 ... 96 take, and lose by it (8464 rows of heads of 80: 444 us with two, 475 with three).
 // Waves of a block: eight share a tile's loads (2 x 4096 rows, heads of 128: 278 us with four, 270 with eight; 4 x 2048 of 256: 163 and 146), but for
 // heads of 72 ... 96, whose tiles do not divide evenly among 512 threads and which vision towers use with short windows (heads of 80: 8464 rows 467 us
 // with four, 543 with eight; windows of 64 rows 64 and 78).
@@ -137,7 +137,8 @@ __device__ __forceinline__ float score(const AttnArgs& a, float s) {
 // which stands in for the columns that q holds zeros for.  All other rows are right as they are, also those that are not a number by a score of their own.
 // One lane a key, over the tiles that this wave worked on; q, lo and hi are the lane's row and its range.
 template <bool BF16, int KC, int CAP>
-__device__ uint32_t spoiled_rows(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int k_lo, int k_hi, int w_lo, int w_hi, int in_lo, int in_hi, int lo, int hi) {
+__device__ uint32_t spoiled_rows(const AttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int k_lo, int k_hi, int w_lo, int w_hi, int in_lo,
+                                 int in_hi, int lo, int hi) {
   constexpr int BK = tile_keys(KC);
   constexpr uint32_t kTop = BF16 ? 0x7f80 : 0x7c00;  // all bits of the exponent
   const int lane = threadIdx.x & 63;
@@ -272,8 +273,8 @@ using const_args = const __attribute__((address_space(4))) AttnArgs;
 // value, 106 when a causal mask hides it from the rows in front of it, 205 in pages beside it.  Not inlined, and with the kernel's arguments read anew:
 // inlined, its scalar registers crowd the loop's (4 x 2048 rows of heads of 256 136 -> 145 us).
 template <bool BF16, int KC, int CAP>
-__attribute__((noinline)) __device__ void mend_rows(const_args* args, uint32_t again_, int b_, int hk_, int pos, int head, int lo, int hi, int k_lo_, int k_hi_, int w_lo_, int w_hi_, int in_lo_,
-                                                    int in_hi_, float* partial_, bool cut_) {
+__attribute__((noinline)) __device__ void mend_rows(const_args* args, uint32_t again_, int b_, int hk_, int pos, int head, int lo, int hi, int k_lo_, int k_hi_,
+                                                    int w_lo_, int w_hi_, int in_lo_, int in_hi_, float* partial_, bool cut_) {
   const uint64_t at = (uint64_t)args;
   const AttnArgs& a = *(const AttnArgs*)(const_args*)((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32 | (uint32_t)uniform((int)at));
   const int b = uniform(b_), hk = uniform(hk_);
@@ -341,10 +342,11 @@ __device__ __forceinline__ float first_lane(float x) { return __int_as_float(uni
 // Tiles are double-buffered: while one is computed the next is on its way from memory to LDS, and one barrier a tile both publishes the
 // arrived one and frees the other (three or four places instead of two: no gain at any width).
 //
-// What bounds it: a SIMD's two waves share the matrix unit and the vector unit, and neither is busy more than half of the time -- reads of LDS, the
-// exchange of maxima and the barrier leave gaps that two waves do not fill; three do not fit the registers.  One MI355X, whose library reaches 1.30
-// PFLOP/s in a large bf16 product: 2 x 4096 rows of 16 heads of 128 254 us (1.08 PFLOP/s), of 64 150 us (0.92), 4 x 2048 rows of 8 heads of 256 over one
-// K/V head 133 us (1.03), 8464 rows of 16 heads of 80 444 us (0.83; the 16-column and 32-column steps round 80 up to 80 and 96).  Tried and not kept: two
+// What bounds it: a SIMD's two waves share the matrix unit and the vector unit (busy 0.51 and 0.45 of the time at 128 columns, 0.46 and 0.58 at 80, 0.45 and
+// 0.29 at 256, 0.40 and 0.63 at 64, where four waves share them) -- reads of LDS, the exchange of maxima and the barrier leave gaps that they do not fill.
+// One MI355X, whose library reaches 1.30 PFLOP/s in a large bf16 product: 2 x 4096 rows of 16 heads of 128 250 us (1.10 PFLOP/s), of 64 146 ... 155 us (0.92),
+// 4 x 2048 rows of 8 heads of 256 over one K/V head 130 us (1.06), 8464 rows of 16 heads of 80 437 us (0.84; the 16-column and 32-column steps round 80 up
+// to 80 and 96).  Tried and not kept: two
 // groups of waves half a tile apart (289 us at 128), the weights of 32 keys beside the products of the next 32 (292), 64 rows a wave
 // (289, and 209 at 256), wave priorities (no change).
 template <bool BF16, int KC, int CAP, int kWaves>
@@ -637,7 +639,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(wav
     }
   }
   const uint64_t bads = __ballot(bad);
-  if (bads) mend_rows<BF16, KC, CAP>((const_args*)__builtin_amdgcn_kernarg_segment_ptr(), (uint32_t)(bads | bads >> 32), b, hk, pos, head, lo_s, hi_s, k_lo, k_hi, w_lo, w_hi, in_lo, in_hi, partial + wave * kWaveRows * (a.dim + 4), partial != nullptr);
+  if (bads)
+    mend_rows<BF16, KC, CAP>((const_args*)__builtin_amdgcn_kernarg_segment_ptr(), (uint32_t)(bads | bads >> 32), b, hk, pos, head, lo_s, hi_s, k_lo, k_hi, w_lo, w_hi,
+                             in_lo, in_hi, partial + wave * kWaveRows * (a.dim + 4), partial != nullptr);
 }
 
 // Joins the runs of keys of the cut tiles: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, join_runs of a wave at a time with the maximum moving as

@@ -659,7 +659,7 @@ def patch_attention(model: Any) -> Dict[str, int]:
     """Run the attention of a transformers encoder through this module, in place: the model's attention function becomes `attention` (with the mask
     of a forward as key ranges), its decoder blocks rotate by positions, its packed vision blocks attend all documents and windows in one launch (the
     framework takes them one by one).  Modules fall back to their own forward for anything the kernels do not take (not on a GPU, autograd on, another
-    type, a mask with holes, dropout of a model in training mode).  -> modules patched per kind.  `unpatch_attention` undoes it."""
+    type, a mask with holes, a mask while a graph is captured, dropout of a model in training mode).  -> modules patched per kind.  `unpatch_attention` undoes it."""
     from transformers import AttentionInterface, AttentionMaskInterface
 
     counts = {"rotary": 0, "decoder": 0, "packed": 0}

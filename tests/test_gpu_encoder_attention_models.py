@@ -204,3 +204,35 @@ def test_calls_that_the_kernel_does_not_take_fall_back(ea):
         want = model(input_ids=x).last_hidden_state
         ea.patch_attention(model)
         assert near(model(input_ids=x, past_key_values=Odd(config=model.config), use_cache=True).last_hidden_state, want)
+
+
+def test_a_patched_decoder_captured_into_a_graph_follows_its_inputs(ea):
+    """Captured once, replayed with new embeddings copied in and eager forwards between the replays.  While capturing the framework hands over a mask, and whether it
+    is one of ranges cannot be asked then: the graph holds the modules' own attention, so it is near the eager forward and the unpatched one, not bit-equal."""
+    model, plain = gemma(), gemma()
+    ea.patch_attention(model)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(2, 33, 128, generator=g, device="cuda").to(torch.bfloat16)
+
+    def body(m=model):
+        return m(inputs_embeds=x, use_cache=False).last_hidden_state
+
+    with torch.inference_mode():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            body()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = body()
+        for _ in range(4):
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+            eager, want = body(), body(plain)
+            got = []
+            for _ in range(2):
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                got.append(out.clone())
+            assert torch.equal(*got) and near(got[0], want) and near(eager, want)

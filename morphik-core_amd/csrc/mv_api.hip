@@ -33,6 +33,7 @@ void set_error(const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   g_err = buf;
+  (void)hipGetLastError();  // what is reported here is not left for the next call on this thread, whose launch check would report it as its own
 }
 
 int hip_fail(hipError_t e, const char* what, const char* file, int line) {
